@@ -235,7 +235,10 @@ def _run_plain(s):
     dy = s["dy"].float()
     if case["keep8"]:
         x = _kept8(x)
-        pre = _kept8(pre) if act != "none" else pre
+        if case["op"] == "gated":  # the groups of each half begin at its start
+            pre = torch.cat([_kept8(pre[:, :n]), _kept8(pre[:, n:])], dim=1)
+        elif act != "none":
+            pre = _kept8(pre)
     if case["op"] == "linear":
         dpre = dy * _slope(pre, act)
     else:
@@ -336,7 +339,10 @@ def exact(case, seed):
     dy = s["dy"].double()
     if case["keep8"]:
         x = _hold8(x)
-        if name != "none":
+        if case["op"] == "gated":
+            a[:, :n] = _hold8(a[:, :n])
+            a[:, n:] = _hold8(a[:, n:])
+        elif name != "none":
             a = _hold8(a)
     if case["op"] == "linear":
         da = dy * df(a)
