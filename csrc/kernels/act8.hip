@@ -1,0 +1,93 @@
+// Activations in 8 bits (the form is in feed_forward.h): pack and unpack.
+//
+// A thread holds eight neighbouring values, four threads a group of 32; the
+// group's largest comes from two exchanges between neighbouring lanes.  One
+// pass over the data, 16 + 8 bytes a thread: bound by memory.
+#include "feed_forward.h"
+#include "linear.h"
+
+namespace ff {
+namespace {
+
+template <typename T>
+__global__ __launch_bounds__(256) void pack_kernel(const Pack p) {
+  const long per = p.ldc / 8, total = p.m * per;  // per is a multiple of 4
+  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total;
+       i += (long)gridDim.x * 256) {
+    const long r = i / per, c = (i - r * per) * 8;
+    float v[8];
+    const T* x = (const T*)p.x + r * p.ldx + c;
+    if (p.vec && c < p.n)
+      load8(x, v);
+    else
+      load_some(x, p.n - c, v);
+    float top = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+      const float u = __builtin_fabsf(v[k]);
+      top = is_finite(v[k]) && u > top ? u : top;
+    }
+    // total is a multiple of 4: a group's four lanes are here together
+    top = fmaxf(top, __shfl_xor(top, 1, 64));
+    top = fmaxf(top, __shfl_xor(top, 2, 64));
+    const int e = scale_exp(top);
+    *(uint2*)(p.codes + i * 8) = encode8(v, e);
+    if ((i & 3) == 0) p.scales[i >> 2] = (unsigned char)(e + 127);
+  }
+}
+
+template <typename T> struct Most;
+template <> struct Most<__bf16> { static constexpr float v = 3.38953139e38f; };
+template <> struct Most<_Float16> { static constexpr float v = 65504.f; };
+template <> struct Most<float> { static constexpr float v = 3.402823466e38f; };
+
+template <typename T>
+__global__ __launch_bounds__(256) void unpack_kernel(const Pack p) {
+  const long per = (p.ldx + 7) / 8, total = p.m * per;
+  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total;
+       i += (long)gridDim.x * 256) {
+    const long r = i / per, c = (i - r * per) * 8;
+    float v[8] = {};
+    if (c < p.n) {  // codes behind n, up to the multiple of 32, are zeros
+      const long at = r * p.ldc + c;
+      decode8(*(const uint2*)(p.codes + at), p.scales[at >> 5], v);
+    }
+    // The largest magnitudes may round up past the type's range: they are
+    // held at its largest value.  NaN fails both comparisons and stays.
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+      v[k] = v[k] > Most<T>::v ? Most<T>::v : v[k];
+      v[k] = v[k] < -Most<T>::v ? -Most<T>::v : v[k];
+    }
+    T* x = (T*)p.x + r * p.ldx + c;
+    if (p.vec)
+      store8(x, v);
+    else
+      store_some(x, p.ldx - c, v);
+  }
+}
+
+}  // namespace
+
+void launch_pack(const Pack& p, hipStream_t st) {
+  const dim3 grid(rocps_grid_for(p.m * (p.ldc / 8), 256, 4096)), block(256);
+  if (p.type == 0)
+    hipLaunchKernelGGL((pack_kernel<__bf16>), grid, block, 0, st, p);
+  else if (p.type == 1)
+    hipLaunchKernelGGL((pack_kernel<_Float16>), grid, block, 0, st, p);
+  else
+    hipLaunchKernelGGL((pack_kernel<float>), grid, block, 0, st, p);
+}
+
+void launch_unpack(const Pack& p, hipStream_t st) {
+  const dim3 grid(rocps_grid_for(p.m * ((p.ldx + 7) / 8), 256, 4096));
+  const dim3 block(256);
+  if (p.type == 0)
+    hipLaunchKernelGGL((unpack_kernel<__bf16>), grid, block, 0, st, p);
+  else if (p.type == 1)
+    hipLaunchKernelGGL((unpack_kernel<_Float16>), grid, block, 0, st, p);
+  else
+    hipLaunchKernelGGL((unpack_kernel<float>), grid, block, 0, st, p);
+}
+
+}  // namespace ff

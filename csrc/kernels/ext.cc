@@ -557,6 +557,8 @@ at::Tensor maxpool332_bwd(at::Tensor dy, at::Tensor idx, long H, long W) {
 
 // ---------------------------------------------------------------------------
 
+void bind_linear(pybind11::module& m);  // linear_ext.cc
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "rocps hand-written CDNA4 (gfx950) kernels";
   m.def("fused_sgd", &fused_sgd);
@@ -576,4 +578,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("conv1x1_wgrad", &conv1x1_wgrad);
   m.def("maxpool332_fwd", &maxpool332_fwd);
   m.def("maxpool332_bwd", &maxpool332_bwd);
+  bind_linear(m);
 }

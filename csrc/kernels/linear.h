@@ -1,0 +1,100 @@
+// Launchers of the linear and the gated layer and of activations in 8 bits.
+// Types: 0 bf16, 1 fp16.  Activations: 0 none, 1 relu, 2 gelu (tanh), 3 silu.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+namespace ff {
+
+// Pitches of operands of the tiled product stay under this many elements, so
+// that a tile's extent is within a 31-bit buffer descriptor.
+constexpr long kMaxPitch = 1L << 22;
+
+// y = act(x W^T + bias) + residual; with `gated`, W = [Wg; Wu] of 2n rows and
+// y = act(x Wg^T + bias[:n]) * (x Wu^T + bias[n:]).
+// x and w: 16-byte aligned, pitch and k in whole 16 bytes.
+struct Forward {
+  int type, act;
+  bool gated;
+  bool vec_out;  // n % 8 == 0 and y, bias, residual 16-byte aligned
+  long m, n, k;
+  const void* x;
+  long ldx;
+  const void* w;
+  long ldw;
+  const void* bias;  // or null
+  const void* res;   // or null
+  long ldr;
+  void* y;  // [m][n]
+  // Pre-activations for the backward pass, or null: 16 bits with rows of
+  // `ldp` (a multiple of 8; of 16 if gated), or codes with rows of `ldp` (a
+  // multiple of 32; of 64) and ldp / 32 scales a row.  The gated layer's up
+  // half begins ldp / 2 on.
+  void* pre;
+  unsigned char* codes;
+  unsigned char* scales;
+  long ldp;
+};
+void launch_linear_forward(const Forward& f, hipStream_t st);
+
+// The gradient of the pre-activations, and its sums over the rows for the
+// bias: g = dy act'(pre), or [dy u act'(g), dy act(g)] for the gated layer.
+struct Slope {
+  int type, act;
+  bool gated;
+  bool vec_dy;  // n % 8 == 0, dy 16-byte aligned with a pitch of such
+  long m, n;
+  const void* dy;
+  long ldy;
+  const void* pre;  // as in Forward, or all null where act is none
+  const unsigned char* codes;
+  const unsigned char* scales;
+  long ldp;
+  void* out;  // [m][ldo], zeros behind each half's n columns; or null
+  long ldo;   // a multiple of 8; the gated layer's up half begins n on
+  float* sums;   // [chunks][n or 2n], or null
+  int chunks;    // rows go to this many runs
+  void* dbias;   // [n or 2n], with sums
+};
+int slope_chunks(long m, long n);
+void launch_slope(const Slope& s, hipStream_t st);
+
+// out[m][n] = sum_k A(m,k) B(n,k) in the operands' type: `a_rows` / `b_rows`
+// say that an operand lies with its rows contiguous (element (r,k) at
+// k * ld + r).  Operands 16-byte aligned with pitches of whole 16 bytes; an
+// operand by k has k in whole 16 bytes, its zeros included.
+struct Matmul {
+  int type;
+  bool a_rows, b_rows;
+  bool vec_out;  // n % 8 == 0, out aligned
+  long m, n, k;
+  const void* a;
+  long lda;
+  const void* b;
+  long ldb;
+  void* out;    // [m][n]
+  float* part;  // [splits][m][n], with splits > 1
+  int splits;
+};
+int matmul_splits(long m, long n, long k);
+void launch_matmul(const Matmul& p, hipStream_t st);
+
+// rows of `n` 16-bit values to rows of `ldo` >= n, zeros behind
+void launch_repack(const void* x, long ldx, long m, long n, void* out,
+                   long ldo, hipStream_t st);
+
+// act8.hip; codes [m][ldc], scales [m][ldc / 32], ldc = n to a multiple of 32
+struct Pack {
+  int type;  // 2: fp32
+  bool vec;  // 16-byte aligned rows, n in whole 16 bytes
+  long m, n;
+  void* x;
+  long ldx;
+  unsigned char* codes;
+  unsigned char* scales;
+  long ldc;
+};
+void launch_pack(const Pack& p, hipStream_t st);
+void launch_unpack(const Pack& p, hipStream_t st);  // zeros to ldx behind n
+
+}  // namespace ff

@@ -1,0 +1,334 @@
+// Torch bindings of the feed-forward kernels: the linear and the gated layer
+// with their gradients, and activations in 8 bits.  Every function checks
+// device, type and shape, works on the device of its input and on that
+// device's current stream, and takes its workspace from torch's allocator.
+#include <torch/extension.h>
+
+#include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
+#include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+
+#include <optional>
+#include <tuple>
+#include <vector>
+
+#include "linear.h"
+
+namespace {
+
+using MaybeTensor = std::optional<at::Tensor>;
+
+hipStream_t stream_of(const at::Tensor& t) {
+  return c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.device().index())
+      .stream();
+}
+
+int type_of(const at::Tensor& t, const char* op) {
+  TORCH_CHECK(t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf,
+              op, ": bfloat16 or float16 on the GPU, got ", t.scalar_type());
+  return t.scalar_type() == at::kBFloat16 ? 0 : 1;
+}
+
+void check_2d(const at::Tensor& t, const at::Tensor& like, const char* op,
+              const char* name) {
+  TORCH_CHECK(t.is_cuda() && t.device() == like.device(), op, ": ", name,
+              " is on ", t.device(), ", not ", like.device());
+  TORCH_CHECK(t.dim() == 2, op, ": ", name, " has ", t.dim(),
+              " dimensions, not 2");
+  TORCH_CHECK(t.scalar_type() == like.scalar_type(), op, ": ", name, " is ",
+              t.scalar_type(), ", not ", like.scalar_type());
+}
+
+long up_to(long n, long to) { return (n + to - 1) / to * to; }
+
+bool aligned(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+// An operand as the tiled product takes it: the tensor itself where its rows
+// are whole 16 bytes, else a copy with zeros behind each row.
+struct Rows {
+  at::Tensor keep;
+  const void* p;
+  long ld;
+};
+
+Rows whole_rows(const at::Tensor& t, hipStream_t st, const char* op) {
+  const long m = t.size(0), n = t.size(1);
+  TORCH_CHECK(n < ff::kMaxPitch, op, ": a row of ", n, " is too long");
+  at::Tensor u = n > 1 && t.stride(1) != 1 ? t.contiguous() : t;
+  const long ld = m > 1 ? u.stride(0) : up_to(n, 8);
+  if (aligned(u.data_ptr()) && n % 8 == 0 && ld % 8 == 0 &&
+      ld < ff::kMaxPitch)
+    return {u, u.data_ptr(), ld};
+  const long ldo = up_to(n, 8);
+  auto out = at::empty({m, ldo}, t.options());
+  ff::launch_repack(u.data_ptr(), m > 1 ? u.stride(0) : n, m, n,
+                    out.data_ptr(), ldo, st);
+  return {out, out.data_ptr(), ldo};
+}
+
+// rows of any alignment, their values side by side
+at::Tensor inner_contiguous(const at::Tensor& t) {
+  return t.size(1) > 1 && t.stride(1) != 1 ? t.contiguous() : t;
+}
+
+}  // namespace
+
+// keep: 0 nothing, 1 the pre-activations in their type, 2 in 8 bits.
+// Returns y, pre or codes, scales.
+std::tuple<at::Tensor, MaybeTensor, MaybeTensor> linear_forward(
+    at::Tensor x, at::Tensor w, MaybeTensor bias, MaybeTensor res, long act,
+    bool gated, long keep) {
+  const char* op = gated ? "gated_linear" : "linear_act";
+  TORCH_CHECK(x.is_cuda(), op, ": x must be on the GPU");
+  ff::Forward f{};
+  f.type = type_of(x, op);
+  check_2d(x, x, op, "x");
+  check_2d(w, x, op, "weight");
+  TORCH_CHECK(act >= 0 && act <= 3 && keep >= 0 && keep <= 2, op,
+              ": unknown activation or checkpoint");
+  TORCH_CHECK(!gated || act != 0, op, ": a gate needs an activation");
+  const long m = x.size(0), k = x.size(1);
+  const long n = gated ? w.size(0) / 2 : w.size(0);
+  TORCH_CHECK(w.size(1) == k, op, ": x has ", k, " features, weight ",
+              w.size(1));
+  TORCH_CHECK(n > 0 && k > 0 && (!gated || w.size(0) % 2 == 0), op,
+              ": weight of ", w.size(0), " x ", w.size(1));
+  c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(x.device());
+  auto st = stream_of(x);
+  auto y = at::empty({m, n}, x.options());
+  f.act = (int)act;
+  f.gated = gated;
+  f.m = m, f.n = n, f.k = k;
+  f.y = y.data_ptr();
+  f.vec_out = n % 8 == 0;
+  at::Tensor b, r;
+  if (bias.has_value()) {
+    TORCH_CHECK(bias->device() == x.device() &&
+                    bias->scalar_type() == x.scalar_type() &&
+                    bias->dim() == 1 && bias->size(0) == w.size(0),
+                op, ": bias must be (", w.size(0), ",) of ", x.scalar_type(),
+                " on ", x.device());
+    b = bias->contiguous();
+    f.bias = b.data_ptr();
+    f.vec_out = f.vec_out && aligned(f.bias);
+  }
+  if (res.has_value()) {
+    TORCH_CHECK(!gated, op, ": no residual");
+    check_2d(*res, x, op, "residual");
+    TORCH_CHECK(res->size(0) == m && res->size(1) == n, op, ": residual of ",
+                res->size(0), " x ", res->size(1), ", not ", m, " x ", n);
+    r = inner_contiguous(*res);
+    f.res = r.data_ptr();
+    f.ldr = m > 1 ? r.stride(0) : n;
+    f.vec_out = f.vec_out && aligned(f.res) && f.ldr % 8 == 0;
+  }
+  MaybeTensor pre, scales;
+  if (keep != 0 && act != 0) {
+    f.ldp = up_to(n, keep == 1 ? 8 : 32) * (gated ? 2 : 1);
+    if (keep == 1) {
+      pre = at::empty({m, f.ldp}, x.options());
+      f.pre = pre->data_ptr();
+    } else {
+      pre = at::empty({m, f.ldp}, x.options().dtype(at::kByte));
+      scales = at::empty({m, f.ldp / 32}, x.options().dtype(at::kByte));
+      f.codes = pre->data_ptr<unsigned char>();
+      f.scales = scales->data_ptr<unsigned char>();
+    }
+  }
+  if (m == 0) return {y, pre, scales};
+  const Rows xr = whole_rows(x, st, op), wr = whole_rows(w, st, op);
+  f.x = xr.p, f.ldx = xr.ld;
+  f.w = wr.p, f.ldw = wr.ld;
+  ff::launch_linear_forward(f, st);
+  return {y, pre, scales};
+}
+
+// The gradients of x, weight and bias, each where asked for.  x: its values,
+// or with `x_scales` their codes; pre: as linear_forward kept them.
+std::tuple<MaybeTensor, MaybeTensor, MaybeTensor> linear_backward(
+    at::Tensor dy, MaybeTensor x, MaybeTensor x_scales, MaybeTensor w,
+    MaybeTensor pre, MaybeTensor scales, long act, bool gated, long k,
+    bool need_x, bool need_w, bool need_b) {
+  const char* op = gated ? "gated_linear" : "linear_act";
+  TORCH_CHECK(dy.is_cuda(), op, ": the gradient must be on the GPU");
+  check_2d(dy, dy, op, "the gradient");
+  const int type = type_of(dy, op);
+  const long m = dy.size(0), n = dy.size(1);
+  const long outs = gated ? 2 * n : n;
+  c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(dy.device());
+  auto st = stream_of(dy);
+  auto opt = dy.options();
+  auto f32 = opt.dtype(at::kFloat);
+  MaybeTensor dx, dw, db;
+  if (need_x) dx = at::empty({m, k}, opt);
+  if (m == 0) {
+    if (need_w) dw = at::zeros({outs, k}, opt);
+    if (need_b) db = at::zeros({outs}, opt);
+    return {dx, dw, db};
+  }
+
+  // ---- the pre-activations' gradient, and its column sums
+  at::Tensor d = inner_contiguous(dy);
+  const bool products = need_x || need_w;
+  ff::Slope s{};
+  s.type = type, s.act = (int)act, s.gated = gated;
+  s.m = m, s.n = n;
+  s.dy = d.data_ptr();
+  s.ldy = m > 1 ? d.stride(0) : up_to(n, 8);
+  s.vec_dy = n % 8 == 0 && aligned(s.dy) && s.ldy % 8 == 0;
+  at::Tensor g, sums;
+  const void* gp = s.dy;
+  long ldg = s.ldy;
+  if (act != 0 || !s.vec_dy || ldg >= ff::kMaxPitch) {
+    ldg = up_to(outs, 8);
+    TORCH_CHECK(ldg < ff::kMaxPitch, op, ": ", outs, " features are too many");
+    if (products) {
+      g = at::empty({m, ldg}, opt);
+      gp = s.out = g.data_ptr();
+      s.ldo = ldg;
+    }
+  }
+  if (act != 0) {
+    TORCH_CHECK(pre.has_value() && pre->is_contiguous() &&
+                    pre->device() == dy.device() && pre->size(0) == m &&
+                    pre->size(1) == up_to(n, scales.has_value() ? 32 : 8) *
+                                        (gated ? 2 : 1),
+                op, ": no pre-activations of this gradient's shape");
+    s.ldp = pre->size(1);
+    if (scales.has_value()) {
+      s.codes = pre->data_ptr<unsigned char>();
+      s.scales = scales->data_ptr<unsigned char>();
+    } else {
+      TORCH_CHECK(pre->scalar_type() == dy.scalar_type(), op, ": gradient of ",
+                  dy.scalar_type(), " for values of ", pre->scalar_type());
+      s.pre = pre->data_ptr();
+    }
+  }
+  s.chunks = ff::slope_chunks(m, n);
+  if (need_b) {
+    db = at::empty({outs}, opt);
+    sums = at::empty({s.chunks, outs}, f32);
+    s.sums = sums.data_ptr<float>();
+    s.dbias = db->data_ptr();
+  }
+  if (s.out != nullptr || need_b) ff::launch_slope(s, st);
+
+  auto product = [&](ff::Matmul& q) {
+    q.type = type;
+    q.vec_out = q.n % 8 == 0;
+    q.splits = ff::matmul_splits(q.m, q.n, q.k);
+    at::Tensor part;
+    if (q.splits > 1) {
+      part = at::empty({q.splits, q.m, q.n}, f32);
+      q.part = part.data_ptr<float>();
+    }
+    ff::launch_matmul(q, st);
+  };
+
+  if (need_x) {
+    TORCH_CHECK(w.has_value() && w->size(0) == outs && w->size(1) == k, op,
+                ": no weight of this gradient's shape");
+    check_2d(*w, dy, op, "weight");
+    const Rows wr = whole_rows(*w, st, op);
+    ff::Matmul q{};
+    q.b_rows = true;
+    q.m = m, q.n = k, q.k = outs;
+    q.a = gp, q.lda = ldg;
+    q.b = wr.p, q.ldb = wr.ld;
+    q.out = dx->data_ptr();
+    product(q);
+  }
+  if (need_w) {
+    TORCH_CHECK(x.has_value(), op, ": no input");
+    Rows xr;
+    if (x_scales.has_value()) {
+      const long ldx = up_to(k, 8), ldc = up_to(k, 32);
+      TORCH_CHECK(x->is_contiguous() && x->size(0) == m && x->size(1) == ldc &&
+                      x->device() == dy.device(),
+                  op, ": no input of this gradient's shape");
+      xr.keep = at::empty({m, ldx}, opt);
+      ff::Pack p{};
+      p.type = type, p.vec = true;
+      p.m = m, p.n = k;
+      p.x = xr.keep.data_ptr(), p.ldx = ldx;
+      p.codes = x->data_ptr<unsigned char>();
+      p.scales = x_scales->data_ptr<unsigned char>();
+      p.ldc = ldc;
+      ff::launch_unpack(p, st);
+      xr.p = p.x, xr.ld = ldx;
+    } else {
+      check_2d(*x, dy, op, "x");
+      TORCH_CHECK(x->size(0) == m && x->size(1) == k, op,
+                  ": no input of this gradient's shape");
+      xr = whole_rows(*x, st, op);
+    }
+    dw = at::empty({outs, k}, opt);
+    ff::Matmul q{};
+    q.a_rows = q.b_rows = true;
+    q.m = outs, q.n = k, q.k = m;
+    q.a = gp, q.lda = ldg;
+    q.b = xr.p, q.ldb = xr.ld;
+    q.out = dw->data_ptr();
+    product(q);
+  }
+  return {dx, dw, db};
+}
+
+static int pack_type(const at::Tensor& t, const char* op) {
+  return t.scalar_type() == at::kFloat ? 2 : type_of(t, op);
+}
+
+// x (m, n) -> codes (m, n to a multiple of 32), scales (m, that / 32)
+std::tuple<at::Tensor, at::Tensor> act8_pack(at::Tensor x) {
+  const char* op = "pack_activation";
+  TORCH_CHECK(x.is_cuda() && x.dim() == 2, op, ": a matrix on the GPU");
+  ff::Pack p{};
+  p.type = pack_type(x, op);
+  c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(x.device());
+  auto v = inner_contiguous(x);
+  p.m = v.size(0), p.n = v.size(1);
+  p.ldc = up_to(p.n, 32);
+  auto codes = at::empty({p.m, p.ldc}, x.options().dtype(at::kByte));
+  auto scales = at::empty({p.m, p.ldc / 32}, x.options().dtype(at::kByte));
+  if (codes.numel() == 0) return {codes, scales};
+  p.x = v.data_ptr();
+  p.ldx = p.m > 1 ? v.stride(0) : p.n;
+  p.vec = aligned(p.x) && p.n % 8 == 0 && p.ldx % 8 == 0;
+  p.codes = codes.data_ptr<unsigned char>();
+  p.scales = scales.data_ptr<unsigned char>();
+  ff::launch_pack(p, stream_of(x));
+  return {codes, scales};
+}
+
+at::Tensor act8_unpack(at::Tensor codes, at::Tensor scales, long n,
+                       at::ScalarType dtype) {
+  const char* op = "unpack_activation";
+  TORCH_CHECK(codes.is_cuda() && codes.device() == scales.device() &&
+                  codes.scalar_type() == at::kByte &&
+                  scales.scalar_type() == at::kByte && codes.dim() == 2 &&
+                  scales.dim() == 2 && codes.is_contiguous() &&
+                  scales.is_contiguous(),
+              op, ": codes and scales as pack_activation gives them");
+  ff::Pack p{};
+  p.m = codes.size(0), p.n = n, p.ldc = codes.size(1);
+  TORCH_CHECK(n >= 0 && p.ldc == up_to(n, 32) && scales.size(0) == p.m &&
+                  scales.size(1) == p.ldc / 32,
+              op, ": codes and scales as pack_activation gives them");
+  c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(codes.device());
+  auto x = at::empty({p.m, n}, codes.options().dtype(dtype));
+  p.type = pack_type(x, op);
+  if (x.numel() == 0) return x;
+  p.x = x.data_ptr();
+  p.ldx = n;
+  p.vec = n % 8 == 0;
+  p.codes = codes.data_ptr<unsigned char>();
+  p.scales = scales.data_ptr<unsigned char>();
+  ff::launch_unpack(p, stream_of(codes));
+  return x;
+}
+
+void bind_linear(pybind11::module& m) {
+  m.def("linear_forward", &linear_forward);
+  m.def("linear_backward", &linear_backward);
+  m.def("act8_pack", &act8_pack);
+  m.def("act8_unpack", &act8_unpack);
+}

@@ -1,0 +1,222 @@
+"""Linear layer with its epilogue: ``y = act(x W^T + b) + r`` in one kernel.
+
+The product runs on the matrix cores with fp32 sums; bias, activation and
+residual are applied to the sums before they are rounded once to the type of
+``x``.  Any number of rows and features, bfloat16 or float16
+(csrc/kernels/linear.hip, linear_rows.hip); on the CPU the same in plain
+PyTorch, in float32 (float64 for float64 inputs).
+
+The backward pass keeps ``x`` and, where there is an activation, the
+pre-activations ``p = x W^T + b`` in the type of ``x``, and computes
+
+    g  = dy * act'(p)              rounded to that type for the products
+    dx = g W      dW = g^T x      db = sum over rows of g      dr = dy
+
+db from the unrounded g.  With ``checkpoint="8bit"`` it keeps x and p in 8
+bits (rocps/ops/act8.py), half the memory: dW and g are then those of the
+kept values; y is the same.
+"""
+
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from rocps.ops import hip_ext, require_hip_for
+from rocps.ops.act8 import pack_rows, unpack_rows
+
+__all__ = ["linear_act"]
+
+_ACTS = {None: 0, "relu": 1, "gelu": 2, "silu": 3}
+_C = 0.7978845608028654  # sqrt(2 / pi)
+_A = 0.044715
+
+
+def act_cpu(v: torch.Tensor, act: int) -> torch.Tensor:
+    if act == 1:
+        return v.clamp(min=0)
+    if act == 2:
+        return 0.5 * v * (1 + torch.tanh(_C * (v + _A * v ** 3)))
+    if act == 3:
+        return v * torch.sigmoid(v)
+    return v
+
+
+def slope_cpu(v: torch.Tensor, act: int) -> torch.Tensor:
+    if act == 1:
+        return (v > 0).to(v.dtype)
+    if act == 2:  # 0 or 1 past 12, where v ** 2 may overflow
+        v = v.clamp(-12, 12)
+        t = torch.tanh(_C * (v + _A * v ** 3))
+        return (0.5 * (1 + t)
+                + 0.5 * v * (1 - t * t) * _C * (1 + 3 * _A * v ** 2))
+    if act == 3:
+        z = torch.sigmoid(v)
+        return z * (1 + v * (1 - z))
+    return torch.ones_like(v)
+
+
+def wide(t: torch.Tensor) -> torch.Tensor:
+    """In the type that the CPU computes in."""
+    return t if t.dtype == torch.float64 else t.float()
+
+
+def check(op: str, x, weight, bias, activation, checkpoint, acts) -> None:
+    """The arguments that both layers share."""
+    if activation not in acts:
+        raise ValueError(f"{op}: activation {activation!r} is not one of "
+                         f"{list(acts)}")
+    if checkpoint not in (None, "8bit"):
+        raise ValueError(f"{op}: checkpoint {checkpoint!r} is not None or "
+                         "'8bit'")
+    if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
+        raise ValueError(f"{op}: x {tuple(x.shape)} and weight "
+                         f"{tuple(weight.shape)} do not fit")
+    if 0 in weight.shape:
+        raise ValueError(f"{op}: weight {tuple(weight.shape)} is empty")
+    if not x.is_floating_point() or (
+            x.is_cuda and x.dtype not in (torch.bfloat16, torch.float16)):
+        raise TypeError(f"{op}: {x.dtype} on {x.device.type}; bfloat16 or "
+                        "float16 on the GPU")
+    if checkpoint is not None and x.dtype == torch.float64:
+        raise TypeError(f"{op}: no 8-bit checkpoint of float64")
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is not None and (t.dtype != x.dtype or t.device != x.device):
+            raise TypeError(f"{op}: {name} is {t.dtype} on {t.device}, x is "
+                            f"{x.dtype} on {x.device}")
+    if bias is not None and bias.shape != weight.shape[:1]:
+        raise ValueError(f"{op}: bias {tuple(bias.shape)}, not "
+                         f"({weight.shape[0]},)")
+
+
+def forward_cpu(x, w, b, r, act: int, gated: bool, keep: int):
+    pre = wide(x) @ wide(w).t()
+    if b is not None:
+        pre = pre + wide(b)
+    if gated:
+        half = pre.shape[1] // 2
+        y = act_cpu(pre[:, :half], act) * pre[:, half:]
+    else:
+        y = act_cpu(pre, act)
+    if r is not None:
+        y = y + wide(r)
+    if keep == 0 or act == 0:
+        return y.to(x.dtype), None, None
+    if keep == 1:
+        return y.to(x.dtype), pre.to(x.dtype), None
+    if gated:  # each half in groups of its own
+        half = pre.shape[1] // 2
+        (g, gs), (u, us) = pack_rows(pre[:, :half]), pack_rows(pre[:, half:])
+        return (y.to(x.dtype), torch.cat([g, u], 1), torch.cat([gs, us], 1))
+    return (y.to(x.dtype), *pack_rows(pre))
+
+
+def backward_cpu(dy, x, x_scales, w, pre, scales, act: int, gated: bool,
+                 k: int, need_x: bool, need_w: bool, need_b: bool):
+    n = dy.shape[1]
+    d = wide(dy)
+    g = d
+    if act != 0:
+        if scales is None:
+            pre = wide(pre)
+        elif gated:
+            c, s = pre.shape[1] // 2, scales.shape[1] // 2
+            pre = torch.cat(
+                [unpack_rows(pre[:, a * c:(a + 1) * c].contiguous(),
+                             scales[:, a * s:(a + 1) * s].contiguous(), n,
+                             torch.float32) for a in (0, 1)], 1)
+        else:
+            pre = unpack_rows(pre, scales, n, torch.float32)
+        if gated:
+            a, u = pre[:, :n], pre[:, n:]
+            g = torch.cat([d * u * slope_cpu(a, act), d * act_cpu(a, act)], 1)
+        else:
+            g = d * slope_cpu(pre, act)
+    dx = dw = db = None
+    if need_x:
+        dx = (g @ wide(w)).to(dy.dtype)
+    if need_w:
+        if x_scales is not None:
+            x = unpack_rows(x, x_scales, k, dy.dtype)
+        dw = (g.t() @ wide(x)).to(dy.dtype)
+    if need_b:
+        db = g.sum(0).to(dy.dtype)
+    return dx, dw, db
+
+
+class LinearFn(torch.autograd.Function):
+    """Both layers on matrices; the gated one has no residual."""
+
+    @staticmethod
+    def forward(ctx, x, w, b, r, act, gated, eight):
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        need = need_x or need_w or need_b
+        fwd = hip_ext().linear_forward if require_hip_for(x) else forward_cpu
+        y, pre, scales = fwd(x, w, b, r, act, gated,
+                             (2 if eight else 1) if need else 0)
+        kept = x_scales = None
+        if need_w:
+            kept, x_scales = pack_rows(x) if eight else (x, None)
+        ctx.save_for_backward(kept, x_scales, w if need_x else None, pre,
+                              scales)
+        ctx.act, ctx.gated, ctx.k = act, gated, x.shape[1]
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, x_scales, w, pre, scales = ctx.saved_tensors
+        bwd = (hip_ext().linear_backward if require_hip_for(dy)
+               else backward_cpu)
+        need = ctx.needs_input_grad
+        dx = dw = db = None
+        if any(need[:3]):
+            dx, dw, db = bwd(dy, x, x_scales, w, pre, scales, ctx.act,
+                             ctx.gated, ctx.k, *need[:3])
+        return dx, dw, db, dy if need[3] else None, None, None, None
+
+
+def apply(x, w, b, r, act: int, gated: bool, eight: bool) -> torch.Tensor:
+    shape = x.shape
+    n = w.shape[0] // 2 if gated else w.shape[0]
+    if len(shape) != 2:
+        x = x.reshape(shape[:-1].numel(), shape[-1])
+        if r is not None:
+            r = r.reshape(x.shape[0], n)
+    if torch.is_grad_enabled() and (
+            x.requires_grad or w.requires_grad
+            or (b is not None and b.requires_grad)
+            or (r is not None and r.requires_grad)):
+        y = LinearFn.apply(x, w, b, r, act, gated, eight)
+    elif require_hip_for(x):
+        y = hip_ext().linear_forward(x, w, b, r, act, gated, 0)[0]
+    else:
+        y = forward_cpu(x, w, b, r, act, gated, 0)[0]
+    return y if len(shape) == 2 else y.reshape(*shape[:-1], n)
+
+
+def linear_act(x: torch.Tensor, weight: torch.Tensor,
+               bias: Optional[torch.Tensor] = None,
+               residual: Optional[torch.Tensor] = None, *,
+               activation: Optional[str] = None,
+               checkpoint: Optional[str] = None) -> torch.Tensor:
+    """``act(x @ weight.T + bias) + residual``.
+
+    x (..., K), weight (N, K), bias (N,), residual (..., N) -> (..., N), all
+    of one type on one device; ``activation`` None, "relu", "gelu" (tanh form)
+    or "silu"; ``checkpoint`` None or "8bit" (see the module).  Rows may have
+    any stride; whole multiples of 8 features from 16-byte aligned rows are
+    used where they lie, others are copied first.  Differentiable once."""
+    check("linear_act", x, weight, bias, activation, checkpoint, _ACTS)
+    if residual is not None:
+        want = x.shape[:-1] + weight.shape[:1]
+        if residual.shape != want:
+            raise ValueError(f"linear_act: residual {tuple(residual.shape)}, "
+                             f"not {tuple(want)}")
+        if residual.dtype != x.dtype or residual.device != x.device:
+            raise TypeError(f"linear_act: residual is {residual.dtype} on "
+                            f"{residual.device}, x is {x.dtype} on {x.device}")
+    return apply(x, weight, bias, residual, _ACTS[activation], False,
+                 checkpoint is not None)

@@ -65,6 +65,10 @@ _hip_sources = [
     "csrc/kernels/maxpool.hip",
     "csrc/kernels/bias_act.hip",
     "csrc/kernels/layernorm.hip",
+    "csrc/kernels/linear_ext.cc",
+    "csrc/kernels/linear.hip",
+    "csrc/kernels/linear_bwd.hip",
+    "csrc/kernels/act8.hip",
 ]
 _hip_sources = [s for s in _hip_sources if os.path.exists(os.path.join(ROOT, s))]
 if _hip_sources:
@@ -78,7 +82,11 @@ if _hip_sources:
                 extra_compile_args={
                     "cxx": ["-O2", "-std=c++17"],
                     "nvcc": ["-O3", "-std=c++17", "--offload-arch=gfx950",
-                             "-fgpu-flush-denormals-to-zero"],
+                             "-fgpu-flush-denormals-to-zero",
+                             # packed fp32 instructions have given wrong
+                             # results on gfx950; plain ones are as fast here
+                             "-Xclang", "-target-feature",
+                             "-Xclang", "-packed-fp32-ops"],
                 },
             ))
     else:  # pragma: no cover — this repo targets ROCm builds only
