@@ -1,6 +1,5 @@
-// What the feed-forward kernels (linear.hip, linear_bwd.hip, linear_rows.hip,
-// act8.hip) share: activations with their slopes, the 8-bit form of
-// activations, and the arguments of the launchers.
+// What the feed-forward kernels share: activations with their slopes, the
+// forms that pre-activations are kept in, and vectors of 16-bit values.
 #pragma once
 
 #include "common.h"
@@ -99,6 +98,24 @@ __device__ __forceinline__ void decode8(uint2 c, unsigned char scale,
   v[6] = p[0] * s, v[7] = p[1] * s;
 }
 
+// ---- pre-activations in 24 bits ---------------------------------------------
+//
+// The gated layer's gradient is a product of both its projections, and each
+// rounded to 16 bits would add as much error to the gradients as their own
+// rounding does.  They are kept as the upper 24 bits of float32 instead: the
+// upper 16 in one plane, the next 8 in another.
+
+__device__ __forceinline__ unsigned to_24(float v) {
+  const unsigned b = __float_as_uint(v);
+  return v != v ? 0x7fc000u : (b + 0x80u) >> 8;
+}
+
+__device__ __forceinline__ float from_24(unsigned hi, unsigned lo) {
+  return __uint_as_float(hi << 16 | lo << 8);
+}
+
+using u16x8 = __attribute__((ext_vector_type(8))) unsigned short;
+
 // ---- 16-bit vectors --------------------------------------------------------
 
 template <typename T> using Vec8 = __attribute__((ext_vector_type(8))) T;
@@ -130,6 +147,29 @@ __device__ __forceinline__ void store_some(T* p, long n, const float* v) {
 #pragma unroll
   for (int k = 0; k < 8; k++)
     if (k < n) p[k] = (T)v[k];
+}
+
+__device__ __forceinline__ void store24(unsigned short* hi, unsigned char* lo,
+                                        const float* v) {
+  u16x8 h;
+  unsigned l[2] = {0, 0};
+#pragma unroll
+  for (int k = 0; k < 8; k++) {
+    const unsigned b = to_24(v[k]);
+    h[k] = (unsigned short)(b >> 8);
+    l[k >> 2] |= (b & 255u) << (k & 3) * 8;
+  }
+  *(u16x8*)hi = h;
+  *(uint2*)lo = make_uint2(l[0], l[1]);
+}
+
+__device__ __forceinline__ void load24(const unsigned short* hi,
+                                       const unsigned char* lo, float* v) {
+  const u16x8 h = *(const u16x8*)hi;
+  const uint2 l = *(const uint2*)lo;
+#pragma unroll
+  for (int k = 0; k < 8; k++)
+    v[k] = from_24(h[k], ((k < 4 ? l.x : l.y) >> (k & 3) * 8) & 255u);
 }
 
 }  // namespace ff

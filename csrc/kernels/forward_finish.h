@@ -1,0 +1,101 @@
+// What follows the products of the forward pass, for eight neighbouring
+// columns of one row: bias, what training keeps, activation, gate, residual
+// and the one rounding to the type.
+#pragma once
+
+#include "feed_forward.h"
+#include "linear.h"
+
+namespace ff {
+
+enum Keep { kNothing = 0, kPre = 1, k8 = 2 };
+
+// columns n.. of the bias, zeros behind the last one
+template <typename T>
+__device__ __forceinline__ void bias8(const Forward& f, long n, long half,
+                                      float* v) {
+  const T* b = (const T*)f.bias;
+  if (b == nullptr || n >= f.n) {
+#pragma unroll
+    for (int k = 0; k < 8; k++) v[k] = 0.f;
+  } else if (f.vec_out) {
+    load8(b + half + n, v);
+  } else {
+    load_some(b + half + n, f.n - n, v);
+  }
+}
+
+// Keeps eight pre-activations of row m, columns n.. of the gated layer's up
+// half or the other.  In 8 bits, the lanes that differ in bits X and Y of
+// their numbers hold one group of 32 columns.
+template <typename T, int KEEP, bool GATED, int X, int Y>
+__device__ __forceinline__ void keep_pre(const Forward& f, long m, long n,
+                                         bool up, bool live, const float* v) {
+  const long at = m * f.ldp + (up ? f.ldp / 2 : 0) + n;
+  if constexpr (KEEP == kPre) {
+    if (live && n < f.n) {
+      if constexpr (GATED)
+        store24((unsigned short*)f.pre + at, f.low + at, v);
+      else
+        store8((T*)f.pre + at, v);
+    }
+  } else if constexpr (KEEP == k8) {
+    float w[8], top = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+      w[k] = n + k < f.n ? v[k] : 0.f;
+      const float u = __builtin_fabsf(w[k]);
+      top = is_finite(w[k]) && u > top ? u : top;
+    }
+    top = fmaxf(top, __shfl_xor(top, X, 64));
+    top = fmaxf(top, __shfl_xor(top, Y, 64));
+    const int e = scale_exp(top);
+    if (live && (n & ~31L) < f.n) {
+      *(uint2*)(f.codes + at) = encode8(w, e);
+      if ((n & 31) == 0) f.scales[at >> 5] = (unsigned char)(e + 127);
+    }
+  }
+}
+
+template <int ACT>
+__device__ __forceinline__ void act8(float* v, int) {
+#pragma unroll
+  for (int k = 0; k < 8; k++) v[k] = act<ACT>(v[k]);
+}
+// ACT < 0: `a` says which
+template <>
+__device__ __forceinline__ void act8<-1>(float* v, int a) {
+  if (a == kGelu) act8<kGelu>(v, a);
+  else if (a == kSilu) act8<kSilu>(v, a);
+  else if (a == kRelu) act8<kRelu>(v, a);
+}
+
+// v (and the gated layer's u): the products, with the bias.  All lanes of a
+// group come here, `live` or not.
+template <typename T, int KEEP, int ACT, bool GATED, int X, int Y>
+__device__ __forceinline__ void finish8(const Forward& f, long m, long n,
+                                        bool live, float* v, float* u) {
+  keep_pre<T, KEEP, GATED, X, Y>(f, m, n, false, live, v);
+  if constexpr (GATED) keep_pre<T, KEEP, GATED, X, Y>(f, m, n, true, live, u);
+  act8<ACT>(v, f.act);
+  if constexpr (GATED) {
+#pragma unroll
+    for (int k = 0; k < 8; k++) v[k] *= u[k];
+  }
+  if (!live || n >= f.n) return;
+  if (!GATED && f.res != nullptr) {
+    if (f.vec_out)
+      load8((const T*)f.res + m * f.ldr + n, u);
+    else
+      load_some((const T*)f.res + m * f.ldr + n, f.n - n, u);
+#pragma unroll
+    for (int k = 0; k < 8; k++) v[k] += u[k];
+  }
+  T* y = (T*)f.y + m * f.n + n;
+  if (f.vec_out)
+    store8(y, v);
+  else
+    store_some(y, f.n - n, v);
+}
+
+}  // namespace ff

@@ -4,6 +4,8 @@
 
 #include <hip/hip_runtime.h>
 
+#include "tile_choice.h"
+
 namespace ff {
 
 // Pitches of operands of the tiled product stay under this many elements, so
@@ -26,16 +28,26 @@ struct Forward {
   const void* res;   // or null
   long ldr;
   void* y;  // [m][n]
-  // Pre-activations for the backward pass, or null: 16 bits with rows of
-  // `ldp` (a multiple of 8; of 16 if gated), or codes with rows of `ldp` (a
-  // multiple of 32; of 64) and ldp / 32 scales a row.  The gated layer's up
-  // half begins ldp / 2 on.
+  // Pre-activations for the backward pass, or all null, with rows of `ldp`:
+  //   linear   pre: 16 bits of the type, ldp a multiple of 8
+  //   gated    pre and low: 24 bits, ldp a multiple of 16
+  //   either   codes and scales: 8 bits, ldp a multiple of 32 (gated: 64) and
+  //            ldp / 32 scales a row
+  // The gated layer's up half begins ldp / 2 on.
   void* pre;
+  unsigned char* low;
   unsigned char* codes;
   unsigned char* scales;
   long ldp;
+  TileChoice choice;
+  float* part;  // [splits][m][n or 2n], with splits > 1
 };
+// Few rows take a kernel of their own, which has no splits.
+bool forward_by_rows(const Forward& f);
+TileChoice forward_choice(const Forward& f);
 void launch_linear_forward(const Forward& f, hipStream_t st);
+void forward_tiles_bf16(const Forward& f, hipStream_t st);
+void forward_tiles_fp16(const Forward& f, hipStream_t st);
 
 // The gradient of the pre-activations, and its sums over the rows for the
 // bias: g = dy act'(pre), or [dy u act'(g), dy act(g)] for the gated layer.
@@ -47,6 +59,7 @@ struct Slope {
   const void* dy;
   long ldy;
   const void* pre;  // as in Forward, or all null where act is none
+  const unsigned char* low;
   const unsigned char* codes;
   const unsigned char* scales;
   long ldp;
@@ -74,10 +87,15 @@ struct Matmul {
   long ldb;
   void* out;    // [m][n]
   float* part;  // [splits][m][n], with splits > 1
-  int splits;
+  TileChoice choice;
 };
-int matmul_splits(long m, long n, long k);
 void launch_matmul(const Matmul& p, hipStream_t st);
+// its tiles alone, to `out` or, with splits > 1, to `part`
+void matmul_tiles_bf16(const Matmul& p, hipStream_t st);
+void matmul_tiles_fp16(const Matmul& p, hipStream_t st);
+// the linear layer's, both operands by k, with splits > 1
+void split_tiles_bf16(const Matmul& p, hipStream_t st);
+void split_tiles_fp16(const Matmul& p, hipStream_t st);
 
 // rows of `n` 16-bit values to rows of `ldo` >= n, zeros behind
 void launch_repack(const void* x, long ldx, long m, long n, void* out,

@@ -9,9 +9,6 @@
 namespace ff {
 namespace {
 
-using tile::Operand;
-using tile::Product;
-
 // ---- the pre-activations' gradient ------------------------------------------
 //
 // A thread owns eight columns and walks down its run of rows; a block is 32
@@ -54,8 +51,13 @@ __global__ __launch_bounds__(256) void slope_kernel(const Slope s) {
             decode8(*(const uint2*)(s.codes + up), s.scales[up >> 5], u);
           }
         } else {
-          load8((const T*)s.pre + at, g);
-          if constexpr (GATED) load8((const T*)s.pre + at + s.ldp / 2, u);
+          if constexpr (GATED) {
+            const long up = at + s.ldp / 2;
+            load24((const unsigned short*)s.pre + at, s.low + at, g);
+            load24((const unsigned short*)s.pre + up, s.low + up, u);
+          } else {
+            load8((const T*)s.pre + at, g);
+          }
         }
       }
 #pragma unroll
@@ -150,67 +152,7 @@ void launch_slope_t(const Slope& s, hipStream_t st) {
   }
 }
 
-// ---- the products -------------------------------------------------------------
-
-template <typename T, int BM, int BN, bool AROWS, bool BROWS, bool SPLIT>
-__global__ __launch_bounds__(256, BM == 256 ? 1 : 2)
-void matmul_kernel(const Matmul q) {
-  using P = Product<T, BM, BN, AROWS, BROWS, false>;
-  __shared__ __attribute__((aligned(1024))) char smem[P::LDS];
-  const int mt = (int)((q.m + BM - 1) / BM), nt = (int)((q.n + BN - 1) / BN);
-  const int tiles = mt * nt;
-  int tm, tn, split = 0;
-  if constexpr (SPLIT) {
-    split = blockIdx.x / tiles;
-    tile::tile_of(blockIdx.x % tiles, tiles, mt, nt, tm, tn);
-  } else {
-    tile::tile_of(blockIdx.x, tiles, mt, nt, tm, tn);
-  }
-  const long m0 = (long)tm * BM, n0 = (long)tn * BN;
-  long k0 = 0, k1 = q.k;
-  if constexpr (SPLIT) {  // runs of whole steps
-    const long steps = (q.k + tile::BK - 1) / tile::BK;
-    k0 = steps * split / q.splits * tile::BK;
-    k1 = steps * (split + 1) / q.splits * tile::BK;
-    if (k1 > q.k) k1 = q.k;
-  }
-  P prod;
-  prod.run(smem, Operand{q.a, q.lda, q.m}, Operand{q.b, q.ldb, q.n}, m0, n0,
-           k0, k1, 0);
-
-  const int lane = threadIdx.x & 63;
-  const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int g = lane >> 4, l = lane & 15;
-#pragma unroll
-  for (int p = 0; p < P::FN / 2; p++) {
-    const long n = n0 + (wid & 1) * P::WN + p * 32 + g * 8;
-#pragma unroll
-    for (int i = 0; i < P::FM; i++) {
-      const long m = m0 + (wid >> 1) * P::WM + i * 16 + l;
-      if (m >= q.m || n >= q.n) continue;
-      if constexpr (SPLIT) {
-        float* o = q.part + ((long)split * q.m + m) * q.n + n;
-        if (q.vec_out) {
-          *(tile::f32x4*)o = prod.acc[i][2 * p];
-          *(tile::f32x4*)(o + 4) = prod.acc[i][2 * p + 1];
-        } else {
-#pragma unroll
-          for (int k = 0; k < 8; k++)
-            if (n + k < q.n) o[k] = prod.acc[i][2 * p + (k >> 2)][k & 3];
-        }
-      } else {
-        float v[8];
-#pragma unroll
-        for (int k = 0; k < 8; k++) v[k] = prod.acc[i][2 * p + (k >> 2)][k & 3];
-        T* o = (T*)q.out + m * q.n + n;
-        if (q.vec_out)
-          store8(o, v);
-        else
-          store_some(o, q.n - n, v);
-      }
-    }
-  }
-}
+// ---- splits of k -------------------------------------------------------------
 
 // sums of the splits, in their order
 template <typename T>
@@ -236,39 +178,6 @@ __global__ __launch_bounds__(256) void join_kernel(const float* part,
           if (i + k < count) v[k] += part[s * count + i + k];
       store_some(out + i, count - i, v);
     }
-  }
-}
-
-template <typename T, int BM, int BN, bool AROWS, bool BROWS>
-void launch_tiles(const Matmul& q, hipStream_t st) {
-  const long tiles = ((q.m + BM - 1) / BM) * ((q.n + BN - 1) / BN);
-  if (q.splits > 1) {
-    hipLaunchKernelGGL((matmul_kernel<T, BM, BN, AROWS, BROWS, true>),
-                       dim3((unsigned)(tiles * q.splits)), dim3(256), 0, st,
-                       q);
-    const long count = q.m * q.n;
-    hipLaunchKernelGGL((join_kernel<T>), dim3(rocps_grid_for(count / 8, 256)),
-                       dim3(256), 0, st, q.part, q.splits, count, (T*)q.out,
-                       q.vec_out);
-  } else {
-    hipLaunchKernelGGL((matmul_kernel<T, BM, BN, AROWS, BROWS, false>),
-                       dim3((unsigned)tiles), dim3(256), 0, st, q);
-  }
-}
-
-bool big_tiles(long m, long n, long k) {
-  return ((m + 255) / 256) * ((n + 255) / 256) >= 192;
-}
-
-template <typename T>
-void launch_matmul_t(const Matmul& q, hipStream_t st) {
-  const bool big = big_tiles(q.m, q.n, q.k);
-  if (q.a_rows) {
-    if (big) launch_tiles<T, 256, 256, true, true>(q, st);
-    else launch_tiles<T, 128, 128, true, true>(q, st);
-  } else {
-    if (big) launch_tiles<T, 256, 256, false, true>(q, st);
-    else launch_tiles<T, 128, 128, false, true>(q, st);
   }
 }
 
@@ -307,18 +216,19 @@ void launch_slope(const Slope& s, hipStream_t st) {
   }
 }
 
-int matmul_splits(long m, long n, long k) {
-  if (big_tiles(m, n, k)) return 1;
-  const long tiles = ((m + 127) / 128) * ((n + 127) / 128);
-  const long steps = (k + tile::BK - 1) / tile::BK;
-  long s = 512 / tiles;               // two blocks on each of 256 CUs
-  if (s > steps / 4) s = steps / 4;   // of four steps at least
-  return (int)(s < 1 ? 1 : s);
-}
-
 void launch_matmul(const Matmul& q, hipStream_t st) {
-  if (q.type == 0) launch_matmul_t<__bf16>(q, st);
-  else launch_matmul_t<_Float16>(q, st);
+  if (q.type == 0) matmul_tiles_bf16(q, st);
+  else matmul_tiles_fp16(q, st);
+  if (q.choice.splits == 1) return;
+  const long count = q.m * q.n;
+  const dim3 grid(rocps_grid_for(count / 8, 256)), block(256);
+  const bool vec = count % 8 == 0;
+  if (q.type == 0)
+    hipLaunchKernelGGL((join_kernel<__bf16>), grid, block, 0, st, q.part,
+                       q.choice.splits, count, (__bf16*)q.out, vec);
+  else
+    hipLaunchKernelGGL((join_kernel<_Float16>), grid, block, 0, st, q.part,
+                       q.choice.splits, count, (_Float16*)q.out, vec);
 }
 
 void launch_repack(const void* x, long ldx, long m, long n, void* out,

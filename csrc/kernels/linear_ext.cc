@@ -55,7 +55,8 @@ Rows whole_rows(const at::Tensor& t, hipStream_t st, const char* op) {
   TORCH_CHECK(n < ff::kMaxPitch, op, ": a row of ", n, " is too long");
   at::Tensor u = n > 1 && t.stride(1) != 1 ? t.contiguous() : t;
   const long ld = m > 1 ? u.stride(0) : up_to(n, 8);
-  if (aligned(u.data_ptr()) && n % 8 == 0 && ld % 8 == 0 &&
+  // ld < n: rows that overlap, as an expanded tensor's
+  if (aligned(u.data_ptr()) && n % 8 == 0 && ld % 8 == 0 && ld >= n &&
       ld < ff::kMaxPitch)
     return {u, u.data_ptr(), ld};
   const long ldo = up_to(n, 8);
@@ -72,8 +73,9 @@ at::Tensor inner_contiguous(const at::Tensor& t) {
 
 }  // namespace
 
-// keep: 0 nothing, 1 the pre-activations in their type, 2 in 8 bits.
-// Returns y, pre or codes, scales.
+// keep: 0 nothing, 1 the pre-activations in their type (the gated layer's in
+// 24 bits: a byte tensor of both planes), 2 in 8 bits.  Returns y, pre or
+// codes, scales.
 std::tuple<at::Tensor, MaybeTensor, MaybeTensor> linear_forward(
     at::Tensor x, at::Tensor w, MaybeTensor bias, MaybeTensor res, long act,
     bool gated, long keep) {
@@ -124,7 +126,11 @@ std::tuple<at::Tensor, MaybeTensor, MaybeTensor> linear_forward(
   MaybeTensor pre, scales;
   if (keep != 0 && act != 0) {
     f.ldp = up_to(n, keep == 1 ? 8 : 32) * (gated ? 2 : 1);
-    if (keep == 1) {
+    if (keep == 1 && gated) {
+      pre = at::empty({m, 3 * f.ldp}, x.options().dtype(at::kByte));
+      f.pre = pre->data_ptr();
+      f.low = pre->data_ptr<unsigned char>() + 2 * m * f.ldp;
+    } else if (keep == 1) {
       pre = at::empty({m, f.ldp}, x.options());
       f.pre = pre->data_ptr();
     } else {
@@ -135,9 +141,19 @@ std::tuple<at::Tensor, MaybeTensor, MaybeTensor> linear_forward(
     }
   }
   if (m == 0) return {y, pre, scales};
+  TORCH_CHECK(m < (1L << 30), op, ": ", m, " rows are too many");
   const Rows xr = whole_rows(x, st, op), wr = whole_rows(w, st, op);
   f.x = xr.p, f.ldx = xr.ld;
   f.w = wr.p, f.ldw = wr.ld;
+  at::Tensor part;
+  if (!ff::forward_by_rows(f)) {
+    f.choice = ff::forward_choice(f);
+    if (f.choice.splits > 1) {
+      part = at::empty({f.choice.splits, m, w.size(0)},
+                       x.options().dtype(at::kFloat));
+      f.part = part.data_ptr<float>();
+    }
+  }
   ff::launch_linear_forward(f, st);
   return {y, pre, scales};
 }
@@ -178,7 +194,7 @@ std::tuple<MaybeTensor, MaybeTensor, MaybeTensor> linear_backward(
   at::Tensor g, sums;
   const void* gp = s.dy;
   long ldg = s.ldy;
-  if (act != 0 || !s.vec_dy || ldg >= ff::kMaxPitch) {
+  if (act != 0 || !s.vec_dy || ldg < n || ldg >= ff::kMaxPitch) {
     ldg = up_to(outs, 8);
     TORCH_CHECK(ldg < ff::kMaxPitch, op, ": ", outs, " features are too many");
     if (products) {
@@ -188,15 +204,18 @@ std::tuple<MaybeTensor, MaybeTensor, MaybeTensor> linear_backward(
     }
   }
   if (act != 0) {
+    const bool eight = scales.has_value();
+    s.ldp = up_to(n, eight ? 32 : 8) * (gated ? 2 : 1);
     TORCH_CHECK(pre.has_value() && pre->is_contiguous() &&
                     pre->device() == dy.device() && pre->size(0) == m &&
-                    pre->size(1) == up_to(n, scales.has_value() ? 32 : 8) *
-                                        (gated ? 2 : 1),
+                    pre->size(1) == s.ldp * (gated && !eight ? 3 : 1),
                 op, ": no pre-activations of this gradient's shape");
-    s.ldp = pre->size(1);
-    if (scales.has_value()) {
+    if (eight) {
       s.codes = pre->data_ptr<unsigned char>();
       s.scales = scales->data_ptr<unsigned char>();
+    } else if (gated) {
+      s.pre = pre->data_ptr<unsigned char>();
+      s.low = pre->data_ptr<unsigned char>() + 2 * m * s.ldp;
     } else {
       TORCH_CHECK(pre->scalar_type() == dy.scalar_type(), op, ": gradient of ",
                   dy.scalar_type(), " for values of ", pre->scalar_type());
@@ -215,10 +234,10 @@ std::tuple<MaybeTensor, MaybeTensor, MaybeTensor> linear_backward(
   auto product = [&](ff::Matmul& q) {
     q.type = type;
     q.vec_out = q.n % 8 == 0;
-    q.splits = ff::matmul_splits(q.m, q.n, q.k);
+    q.choice = ff::choose_tile(q.m, q.n, q.k, false);
     at::Tensor part;
-    if (q.splits > 1) {
-      part = at::empty({q.splits, q.m, q.n}, f32);
+    if (q.choice.splits > 1) {
+      part = at::empty({q.choice.splits, q.m, q.n}, f32);
       q.part = part.data_ptr<float>();
     }
     ff::launch_matmul(q, st);

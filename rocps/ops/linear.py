@@ -12,7 +12,9 @@ pre-activations ``p = x W^T + b`` in the type of ``x``, and computes
     g  = dy * act'(p)              rounded to that type for the products
     dx = g W      dW = g^T x      db = sum over rows of g      dr = dy
 
-db from the unrounded g.  With ``checkpoint="8bit"`` it keeps x and p in 8
+(the gated layer keeps its two projections in 24 bits: g is a product of both,
+and their rounding to 16 would add as much error as that of g itself);
+db is taken from the unrounded g.  With ``checkpoint="8bit"`` it keeps x and p in 8
 bits (rocps/ops/act8.py), half the memory: dW and g are then those of the
 kept values; y is the same.
 """
@@ -104,8 +106,8 @@ def forward_cpu(x, w, b, r, act: int, gated: bool, keep: int):
         y = y + wide(r)
     if keep == 0 or act == 0:
         return y.to(x.dtype), None, None
-    if keep == 1:
-        return y.to(x.dtype), pre.to(x.dtype), None
+    if keep == 1:  # the gated layer's in more than 16 bits, see the module
+        return y.to(x.dtype), pre if gated else pre.to(x.dtype), None
     if gated:  # each half in groups of its own
         half = pre.shape[1] // 2
         (g, gs), (u, us) = pack_rows(pre[:, :half]), pack_rows(pre[:, half:])

@@ -66,8 +66,12 @@ _hip_sources = [
     "csrc/kernels/bias_act.hip",
     "csrc/kernels/layernorm.hip",
     "csrc/kernels/linear_ext.cc",
-    "csrc/kernels/linear.hip",
+    "csrc/kernels/linear_fwd_bf16.hip",
+    "csrc/kernels/linear_fwd_fp16.hip",
+    "csrc/kernels/linear_rows.hip",
     "csrc/kernels/linear_bwd.hip",
+    "csrc/kernels/tile_matmul_bf16.hip",
+    "csrc/kernels/tile_matmul_fp16.hip",
     "csrc/kernels/act8.hip",
 ]
 _hip_sources = [s for s in _hip_sources if os.path.exists(os.path.join(ROOT, s))]
