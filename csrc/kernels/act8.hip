@@ -21,17 +21,9 @@ __global__ __launch_bounds__(256) void pack_kernel(const Pack p) {
       load8(x, v);
     else
       load_some(x, p.n - c, v);
-    float top = 0.f;
-#pragma unroll
-    for (int k = 0; k < 8; k++) {
-      const float u = __builtin_fabsf(v[k]);
-      top = is_finite(v[k]) && u > top ? u : top;
-    }
     // total is a multiple of 4: a group's four lanes are here together
-    top = fmaxf(top, __shfl_xor(top, 1, 64));
-    top = fmaxf(top, __shfl_xor(top, 2, 64));
-    const int e = scale_exp(top);
-    *(uint2*)(p.codes + i * 8) = encode8(v, e);
+    int e;
+    *(uint2*)(p.codes + i * 8) = encode8<1, 2>(v, e);
     if ((i & 3) == 0) p.scales[i >> 2] = (unsigned char)(e + 127);
   }
 }

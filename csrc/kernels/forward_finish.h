@@ -26,8 +26,8 @@ __device__ __forceinline__ void bias8(const Forward& f, long n, long half,
 }
 
 // Keeps eight pre-activations of row m, columns n.. of the gated layer's up
-// half or the other.  In 8 bits, the lanes that differ in bits X and Y of
-// their numbers hold one group of 32 columns.
+// half or the other.  In 8 bits, the lanes X, Y and X + Y away hold the
+// rest of a group of 32 columns.
 template <typename T, int KEEP, bool GATED, int X, int Y>
 __device__ __forceinline__ void keep_pre(const Forward& f, long m, long n,
                                          bool up, bool live, const float* v) {
@@ -40,18 +40,14 @@ __device__ __forceinline__ void keep_pre(const Forward& f, long m, long n,
         store8((T*)f.pre + at, v);
     }
   } else if constexpr (KEEP == k8) {
-    float w[8], top = 0.f;
+    float w[8];
+    const bool whole = n + 8 <= f.n;
 #pragma unroll
-    for (int k = 0; k < 8; k++) {
-      w[k] = n + k < f.n ? v[k] : 0.f;
-      const float u = __builtin_fabsf(w[k]);
-      top = is_finite(w[k]) && u > top ? u : top;
-    }
-    top = fmaxf(top, __shfl_xor(top, X, 64));
-    top = fmaxf(top, __shfl_xor(top, Y, 64));
-    const int e = scale_exp(top);
+    for (int k = 0; k < 8; k++) w[k] = whole || n + k < f.n ? v[k] : 0.f;
+    int e;
+    const uint2 codes = encode8<X, Y>(w, e);
     if (live && (n & ~31L) < f.n) {
-      *(uint2*)(f.codes + at) = encode8(w, e);
+      *(uint2*)(f.codes + at) = codes;
       if ((n & 31) == 0) f.scales[at >> 5] = (unsigned char)(e + 127);
     }
   }
@@ -70,27 +66,38 @@ __device__ __forceinline__ void act8<-1>(float* v, int a) {
   else if (a == kRelu) act8<kRelu>(v, a);
 }
 
-// v (and the gated layer's u): the products, with the bias.  All lanes of a
-// group come here, `live` or not.
+// Eight columns of the residual, zeros where there is none.
+template <typename T>
+__device__ __forceinline__ Vec8<T> residual8(const Forward& f, long m, long n) {
+  Vec8<T> r = {};
+  if (f.res != nullptr && m < f.m && n < f.n) {
+    const T* p = (const T*)f.res + m * f.ldr + n;
+    if (f.vec_out) {
+      r = *(const Vec8<T>*)p;
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; k++)
+        if (n + k < f.n) r[k] = p[k];
+    }
+  }
+  return r;
+}
+
+// v (and the gated layer's u): the products, with the bias; r: the residual.
+// All lanes of a group come here, `live` or not.
 template <typename T, int KEEP, int ACT, bool GATED, int X, int Y>
 __device__ __forceinline__ void finish8(const Forward& f, long m, long n,
-                                        bool live, float* v, float* u) {
+                                        bool live, float* v, float* u,
+                                        Vec8<T> r) {
   keep_pre<T, KEEP, GATED, X, Y>(f, m, n, false, live, v);
   if constexpr (GATED) keep_pre<T, KEEP, GATED, X, Y>(f, m, n, true, live, u);
   act8<ACT>(v, f.act);
-  if constexpr (GATED) {
 #pragma unroll
-    for (int k = 0; k < 8; k++) v[k] *= u[k];
+  for (int k = 0; k < 8; k++) {
+    if constexpr (GATED) v[k] *= u[k];
+    else v[k] += (float)r[k];
   }
   if (!live || n >= f.n) return;
-  if (!GATED && f.res != nullptr) {
-    if (f.vec_out)
-      load8((const T*)f.res + m * f.ldr + n, u);
-    else
-      load_some((const T*)f.res + m * f.ldr + n, f.n - n, u);
-#pragma unroll
-    for (int k = 0; k < 8; k++) v[k] += u[k];
-  }
   T* y = (T*)f.y + m * f.n + n;
   if (f.vec_out)
     store8(y, v);

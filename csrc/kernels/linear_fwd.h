@@ -19,8 +19,22 @@ __device__ __forceinline__ void finish(const P& prod, const Forward& f,
   const int lane = threadIdx.x & 63;
   const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   constexpr int COLS = GATED ? P::WN / 2 : P::WN;
+  // The whole residual before the first store, which the compiler has to take
+  // for one to the same place: one wait instead of one a row.  Its registers
+  // are the fragments'.
+  constexpr int PAIRS = COLS / 32;
+  Vec8<T> r[GATED ? 1 : PAIRS][P::FM] = {};
+  if constexpr (!GATED) {
 #pragma unroll
-  for (int p = 0; p < COLS / 32; p++) {
+    for (int p = 0; p < PAIRS; p++)
+#pragma unroll
+      for (int i = 0; i < P::FM; i++)
+        r[p][i] = residual8<T>(
+            f, m0 + (wid >> 1) * P::WM + i * 16 + (lane & 15),
+            n0 + (wid & 1) * COLS + p * 32 + P::column(lane));
+  }
+#pragma unroll
+  for (int p = 0; p < PAIRS; p++) {
     const long n = n0 + (wid & 1) * COLS + p * 32 + P::column(lane);
     float b[8], bu[8];
     bias8<T>(f, n, 0, b);
@@ -37,7 +51,8 @@ __device__ __forceinline__ void finish(const P& prod, const Forward& f,
 #pragma unroll
         for (int k = 0; k < 8; k++) u[k] += bu[k];
       }
-      finish8<T, KEEP, ACT, GATED, 16, 32>(f, m, n, m < f.m, v, u);
+      finish8<T, KEEP, ACT, GATED, 16, 32>(f, m, n, m < f.m, v, u,
+                                           r[GATED ? 0 : p][i]);
     }
   }
 }

@@ -86,6 +86,8 @@ __global__ __launch_bounds__(64 * kWaves) void rows_kernel(const Forward f) {
   float v[8], u[8];
   bias8<T>(f, n0 + c, 0, v);
   if constexpr (GATED) bias8<T>(f, n0 + c, f.n, u);
+  Vec8<T> r = {};
+  if constexpr (!GATED) r = residual8<T>(f, m, n0 + c);
 #pragma unroll
   for (int s = 0; s < kWaves; s++)
 #pragma unroll
@@ -100,7 +102,7 @@ __global__ __launch_bounds__(64 * kWaves) void rows_kernel(const Forward f) {
         for (int r = 0; r < 4; r++) u[q * 4 + r] += o[r];
       }
     }
-  finish8<T, KEEP, -1, GATED, 1, 2>(f, m, n0 + c, m < f.m, v, u);
+  finish8<T, KEEP, -1, GATED, 1, 2>(f, m, n0 + c, m < f.m, v, u, r);
 }
 
 template <typename T, int MF, bool GATED>
@@ -136,6 +138,8 @@ __global__ __launch_bounds__(256) void join_forward_kernel(const Forward f) {
     float v[8], u[8];
     bias8<T>(f, n, 0, v);
     if constexpr (GATED) bias8<T>(f, n, f.n, u);
+    Vec8<T> r = {};
+    if constexpr (!GATED) r = residual8<T>(f, m, n);
     for (int s = 0; s < f.choice.splits; s++) {
       const float* p = f.part + ((long)s * f.m + m) * width + n;
       if (vec && n < f.n) {
@@ -159,7 +163,7 @@ __global__ __launch_bounds__(256) void join_forward_kernel(const Forward f) {
           }
       }
     }
-    finish8<T, KEEP, -1, GATED, 1, 2>(f, m, n, true, v, u);
+    finish8<T, KEEP, -1, GATED, 1, 2>(f, m, n, true, v, u, r);
   }
 }
 

@@ -179,15 +179,15 @@ __device__ __forceinline__ void barrier() {
 // 16 bytes a lane from memory to LDS at `dst` + 16 lane; `dst` is the wave's.
 // As an instruction, because before a transposing read of LDS the compiler
 // waits for every such load that it knows of.  It has no register to write,
-// and `wait` is what waits for it.
+// and `wait` is what waits for it.  M0, which it takes the place from, is the
+// compiler's only around instructions that these kernels do not have.
 __device__ __forceinline__ void load_lds(Descriptor r, lds_char* dst,
                                          unsigned off, int soff) {
   asm volatile(
       "s_mov_b32 m0, %0\n\ts_nop 0\n\t"
       "buffer_load_dwordx4 %1, %2, %3 offen lds"
       :
-      : "s"((unsigned)(unsigned long)dst), "v"(off), "s"(r), "s"(soff)
-      : "m0");
+      : "s"((unsigned)(unsigned long)dst), "v"(off), "s"(r), "s"(soff));
 }
 
 // Blocks go round the 8 XCDs by their number; giving each XCD a run of
@@ -398,42 +398,44 @@ struct Product {
       else
         f[j] = *(lds_v8*)(t + (boff[0] ^ (kk << 6)) + j * 2048);
     };
-    // The products of 32 k's, of ua and ub, row of blocks by row.  Between the
-    // rows: one operand's loads, and the next 32's reads into na and nb, B's
-    // fragments first, which every row needs.  The last rows are left without
-    // reads, which the wait then finds done.
-    constexpr int READS = FM + FN;
-    constexpr int RGROUPS = FM > 4 ? FM - 2 : FM - 1;
-    constexpr int RPG = (READS + RGROUPS - 1) / RGROUPS;
+    // The products of 32 k's, of ua and ub.  A matrix instruction keeps its
+    // pipe busy for 16 clocks and the wave for 4: what else there is to issue
+    // goes in between, one at a time.  That is the next 32's reads into na and
+    // nb (B's fragments first, which every row of blocks needs; none in the
+    // last quarter, so that the wait finds them done) and one operand's loads.
+    constexpr int READS = FM + FN, SLOTS = FM * FN;
     auto half = [&](const i16x8(&ua)[FM], const i16x8(&ub)[FN],
                     i16x8(&na)[FM], i16x8(&nb)[FN], lds_char* ra,
                     lds_char* rb, int kk, bool b_loads, lds_char* to) {
       const int loads = b_loads ? SB::PASSES : SA::PASSES;
-      const int lpg = (loads + FM - 1) / FM;
       const Source src = b_loads ? source_b() : source_a();
 #pragma unroll
-      for (int i = 0; i < FM; i++) {
+      for (int i = 0; i < FM; i++)
 #pragma unroll
-        for (int q = i * lpg; q < (i + 1) * lpg && q < loads; q++) {
-          if (b_loads)
-            load_b(src, to, q);
-          else
-            load_a(src, to, q);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int x = i * RPG; x < (i + 1) * RPG && x < READS; x++) {
-          if (x < FN)
-            read_b(nb, x, rb, kk);
-          else
-            read_a(na, x - FN, ra, kk);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int j = 0; j < FN; j++)
+        for (int j = 0; j < FN; j++) {
+          const int slot = i * FN + j;
           mfma<T, AGPR>(acc[i][j], ub[j], ua[i]);
-        __builtin_amdgcn_sched_barrier(0);
-      }
+          __builtin_amdgcn_sched_barrier(0);
+          // the reads and loads that fall due by the end of this slot
+#pragma unroll
+          for (int x = slot * READS * 4 / (SLOTS * 3);
+               x < (slot + 1) * READS * 4 / (SLOTS * 3) && x < READS;
+               x++) {
+            if (x < FN)
+              read_b(nb, x, rb, kk);
+            else
+              read_a(na, x - FN, ra, kk);
+          }
+#pragma unroll
+          for (int q = slot * loads / SLOTS; q < (slot + 1) * loads / SLOTS;
+               q++) {
+            if (b_loads)
+              load_b(src, to, q);
+            else
+              load_a(src, to, q);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
     };
 
 #pragma unroll
