@@ -2,6 +2,7 @@
 // with their gradients, and activations in 8 bits.  Every function checks
 // device, type and shape, works on the device of its input and on that
 // device's current stream, and takes its workspace from torch's allocator.
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
@@ -234,7 +235,7 @@ std::tuple<MaybeTensor, MaybeTensor, MaybeTensor> linear_backward(
   auto product = [&](ff::Matmul& q) {
     q.type = type;
     q.vec_out = q.n % 8 == 0;
-    q.choice = ff::choose_tile(q.m, q.n, q.k, false);
+    q.choice = ff::choose_tile(q.m, q.n, q.k);
     at::Tensor part;
     if (q.choice.splits > 1) {
       part = at::empty({q.choice.splits, q.m, q.n}, f32);
@@ -345,7 +346,143 @@ at::Tensor act8_unpack(at::Tensor codes, at::Tensor scales, long n,
   return x;
 }
 
+// ---- the layers, with autograd -------------------------------------------------
+
+namespace {
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+MaybeTensor maybe(const at::Tensor& t) {
+  return t.defined() ? MaybeTensor(t) : std::nullopt;
+}
+
+// In C++, so that a step of a small layer is not one of Python's.
+struct LayerFunction : torch::autograd::Function<LayerFunction> {
+  static at::Tensor forward(AutogradContext* ctx, at::Tensor x, at::Tensor w,
+                            MaybeTensor b, MaybeTensor r, int64_t act,
+                            bool gated, bool eight) {
+    const bool need_x = x.requires_grad(), need_w = w.requires_grad();
+    const bool need = need_x || need_w || (b && b->requires_grad());
+    auto [y, pre, scales] = linear_forward(x, w, b, r, act, gated,
+                                           need ? (eight ? 2 : 1) : 0);
+    at::Tensor kept, kept_scales;
+    if (need_w) {
+      if (eight)
+        std::tie(kept, kept_scales) = act8_pack(x);
+      else
+        kept = x;
+    }
+    ctx->save_for_backward({kept, kept_scales, need_x ? w : at::Tensor(),
+                            pre.value_or(at::Tensor()),
+                            scales.value_or(at::Tensor())});
+    ctx->saved_data["act"] = act;
+    ctx->saved_data["gated"] = gated;
+    ctx->saved_data["k"] = x.size(1);
+    ctx->saved_data["bias"] = b.has_value();
+    ctx->saved_data["residual"] = r.has_value();
+    return y;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const auto& dy = grads[0];
+    const bool need_x = ctx->needs_input_grad(0);
+    const bool need_w = ctx->needs_input_grad(1);
+    // counted among the tensors that there are
+    const bool b = ctx->saved_data["bias"].toBool();
+    const bool r = ctx->saved_data["residual"].toBool();
+    const bool need_b = b && ctx->needs_input_grad(2);
+    const bool need_r = r && ctx->needs_input_grad(b ? 3 : 2);
+    variable_list out(7);
+    if (!dy.defined()) return out;
+    if (need_x || need_w || need_b) {
+      at::NoGradGuard no_grad;
+      auto [dx, dw, db] = linear_backward(
+          dy, maybe(saved[0]), maybe(saved[1]), maybe(saved[2]),
+          maybe(saved[3]), maybe(saved[4]), ctx->saved_data["act"].toInt(),
+          ctx->saved_data["gated"].toBool(), ctx->saved_data["k"].toInt(),
+          need_x, need_w, need_b);
+      out[0] = dx.value_or(at::Tensor());
+      out[1] = dw.value_or(at::Tensor());
+      out[2] = db.value_or(at::Tensor());
+    }
+    if (need_r) out[3] = dy;
+    if (at::GradMode::is_enabled()) {
+      // these gradients are constants to autograd; a second derivative
+      // through them would be wrong, so it raises
+      for (int i = 0; i < 3; i++)
+        if (out[i].defined()) {
+          auto fail = std::make_shared<torch::autograd::DelayedError>(
+              "linear_act and gated_linear are differentiable once", 1);
+          auto v = out[i].detach();
+          v.set_requires_grad(true);
+          out[i] = (*fail)({v})[0];
+        }
+    }
+    return out;
+  }
+};
+
+}  // namespace
+
+// The layer of rocps/ops/linear.py (or gated.py) for x of any leading axes.
+at::Tensor linear_layer(at::Tensor x, at::Tensor w, MaybeTensor bias,
+                        MaybeTensor res, long act, bool gated, bool eight) {
+  const char* op = gated ? "gated_linear" : "linear_act";
+  TORCH_CHECK_VALUE(x.dim() >= 1 && w.dim() == 2 && x.size(-1) == w.size(1),
+                    op, ": x ", x.sizes(), " and weight ", w.sizes(),
+                    " do not fit");
+  TORCH_CHECK_VALUE(w.numel() > 0, op, ": weight ", w.sizes(), " is empty");
+  TORCH_CHECK_VALUE(!gated || w.size(0) % 2 == 0, op, ": weight ", w.sizes(),
+                    " has no two halves");
+  TORCH_CHECK_TYPE(x.scalar_type() == at::kBFloat16 ||
+                       x.scalar_type() == at::kHalf,
+                   op, ": ", x.scalar_type(),
+                   " on the GPU; bfloat16 or float16 there");
+  auto same = [&](const at::Tensor& t, const char* name) {
+    TORCH_CHECK_TYPE(t.scalar_type() == x.scalar_type() &&
+                         t.device() == x.device(),
+                     op, ": ", name, " is ", t.scalar_type(), " on ",
+                     t.device(), ", x is ", x.scalar_type(), " on ",
+                     x.device());
+  };
+  same(w, "weight");
+  if (bias.has_value()) {
+    same(*bias, "bias");
+    TORCH_CHECK_VALUE(bias->dim() == 1 && bias->size(0) == w.size(0), op,
+                      ": bias ", bias->sizes(), ", not (", w.size(0), ",)");
+  }
+  const long n = gated ? w.size(0) / 2 : w.size(0);
+  auto shape = x.sizes().vec();
+  shape.back() = n;
+  if (res.has_value()) {
+    same(*res, "residual");
+    TORCH_CHECK_VALUE(res->sizes() == at::IntArrayRef(shape), op,
+                      ": residual ", res->sizes(), ", not ",
+                      at::IntArrayRef(shape));
+  }
+  const bool flat = x.dim() == 2;
+  long m = 1;
+  for (int i = 0; i + 1 < x.dim(); i++) m *= x.size(i);
+  if (!flat) {
+    x = x.reshape({m, x.size(-1)});
+    if (res.has_value()) res = res->reshape({m, n});
+  }
+  auto grad = [](const MaybeTensor& t) {
+    return t.has_value() && t->requires_grad();
+  };
+  at::Tensor y;
+  if (at::GradMode::is_enabled() && (x.requires_grad() || w.requires_grad() ||
+                                     grad(bias) || grad(res)))
+    y = LayerFunction::apply(x, w, bias, res, (int64_t)act, gated, eight);
+  else
+    y = std::get<0>(linear_forward(x, w, bias, res, act, gated, 0));
+  return flat ? y : y.view(shape);
+}
+
 void bind_linear(pybind11::module& m) {
+  m.def("linear_layer", &linear_layer);
   m.def("linear_forward", &linear_forward);
   m.def("linear_backward", &linear_backward);
   m.def("act8_pack", &act8_pack);

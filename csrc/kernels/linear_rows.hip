@@ -190,7 +190,8 @@ bool forward_by_rows(const Forward& f) {
 }
 
 TileChoice forward_choice(const Forward& f) {
-  return choose_tile(f.m, f.gated ? 2 * f.n : f.n, f.k, f.gated);
+  return choose_tile(f.m, f.gated ? 2 * f.n : f.n, f.k, f.gated,
+                     f.codes != nullptr ? 2 : f.pre != nullptr ? 1 : 0);
 }
 
 void launch_linear_forward(const Forward& f, hipStream_t st) {

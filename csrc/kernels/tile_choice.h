@@ -7,9 +7,11 @@
 //   256 x 256    1        1.40         1.40            13
 //   256 x 128    1        0.80         0.80            15
 //   128 x 192    1        0.61         0.61            14
-//   128 x 128    2        0.45         0.42             9
+//   128 x 128    2        0.50         0.42             9
 //    64 x 128    2        0.36         0.27            12
 //    64 x  64    4        0.34         0.17             8
+// and with pre-activations kept, 3 more where one block has the CU and 5 more
+// where they share it; in 8 bits 9 and 8 more.
 // A larger tile does more with what it reads; a smaller one leaves fewer CUs
 // without work at the end, and two blocks on a CU write one's results while
 // they multiply the other's.  The choice is the least time of the fullest CU.
@@ -30,10 +32,12 @@ struct TileChoice {
 };
 
 // `halves`: the gated layer's, whose tiles hold two runs of whole 32 columns.
-inline TileChoice choose_tile(long m, long n, long k, bool halves) {
+// `keep`: what is kept, 0 nothing, 1 pre-activations, 2 those in 8 bits.
+inline TileChoice choose_tile(long m, long n, long k, bool halves = false,
+                              int keep = 0) {
   struct { long bm, bn; int per_cu; double alone, each, out; } const t[kTiles] =
       {{256, 256, 1, 1.40, 1.40, 13}, {256, 128, 1, 0.80, 0.80, 15},
-       {128, 192, 1, 0.61, 0.61, 14}, {128, 128, 2, 0.45, 0.42, 9},
+       {128, 192, 1, 0.61, 0.61, 14}, {128, 128, 2, 0.50, 0.42, 9},
        {64, 128, 2, 0.36, 0.27, 12},  {64, 64, 4, 0.34, 0.17, 8}};
   const long cus = 256;
   const long steps = (k + 63) / 64;
@@ -43,7 +47,10 @@ inline TileChoice choose_tile(long m, long n, long k, bool halves) {
     if (halves && (t[i].bn == 192 || t[i].bn == 64)) continue;
     const long tiles = ((m + t[i].bm - 1) / t[i].bm) *
                        ((n + t[i].bn - 1) / t[i].bn);
-    const double out = t[i].out * t[i].bm * t[i].bn / 65536;
+    const double more = keep == 0 ? 0
+                        : t[i].per_cu == 1 ? (keep == 1 ? 3 : 9)
+                                           : (keep == 1 ? 5 : 8);
+    const double out = (t[i].out + more) * t[i].bm * t[i].bn / 65536;
     for (int s = 1; s <= 16 && (s == 1 || s * 4 <= steps); s++) {
       const long each = (tiles * s + cus - 1) / cus;  // of the fullest CU
       const long rest = each % t[i].per_cu;

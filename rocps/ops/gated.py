@@ -21,7 +21,7 @@ from typing import Optional
 
 import torch
 
-from rocps.ops.linear import _ACTS, apply, check
+from rocps.ops.linear import _ACTS, layer
 
 __all__ = ["gated_linear"]
 
@@ -34,9 +34,5 @@ def gated_linear(x: torch.Tensor, weight: torch.Tensor,
                  checkpoint: Optional[str] = None) -> torch.Tensor:
     """x (..., K), weight (2 F, K), bias (2 F,) -> (..., F), all of one type on
     one device; ``activation`` "silu", "gelu" (tanh form) or "relu"."""
-    check("gated_linear", x, weight, bias, activation, checkpoint, _GATES)
-    if weight.shape[0] % 2:
-        raise ValueError(f"gated_linear: weight {tuple(weight.shape)} has no "
-                         "two halves")
-    return apply(x, weight, bias, None, _GATES[activation], True,
-                 checkpoint is not None)
+    return layer("gated_linear", _GATES, x, weight, bias, None, activation,
+                 checkpoint, True)

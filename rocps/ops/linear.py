@@ -3,7 +3,8 @@
 The product runs on the matrix cores with fp32 sums; bias, activation and
 residual are applied to the sums before they are rounded once to the type of
 ``x``.  Any number of rows and features, bfloat16 or float16
-(csrc/kernels/linear.hip, linear_rows.hip); on the CPU the same in plain
+(csrc/kernels/linear_fwd.h, linear_rows.hip, linear_bwd.hip on the product of
+tile_gemm.h); on the CPU the same in plain
 PyTorch, in float32 (float64 for float64 inputs).
 
 The backward pass keeps ``x`` and, where there is an activation, the
@@ -12,10 +13,10 @@ pre-activations ``p = x W^T + b`` in the type of ``x``, and computes
     g  = dy * act'(p)              rounded to that type for the products
     dx = g W      dW = g^T x      db = sum over rows of g      dr = dy
 
-(the gated layer keeps its two projections in 24 bits: g is a product of both,
-and their rounding to 16 would add as much error as that of g itself);
-db is taken from the unrounded g.  With ``checkpoint="8bit"`` it keeps x and p in 8
-bits (rocps/ops/act8.py), half the memory: dW and g are then those of the
+db from the unrounded g.  (The gated layer keeps its two projections in 24
+bits: g is a product of both, and their rounding to 16 would add as much error
+as that of g itself.)  With ``checkpoint="8bit"`` it keeps x and p in 8 bits
+(rocps/ops/act8.py), half the memory or less: dW and g are then those of the
 kept values; y is the same.
 """
 
@@ -65,24 +66,15 @@ def wide(t: torch.Tensor) -> torch.Tensor:
     return t if t.dtype == torch.float64 else t.float()
 
 
-def check(op: str, x, weight, bias, activation, checkpoint, acts) -> None:
-    """The arguments that both layers share."""
-    if activation not in acts:
-        raise ValueError(f"{op}: activation {activation!r} is not one of "
-                         f"{list(acts)}")
-    if checkpoint not in (None, "8bit"):
-        raise ValueError(f"{op}: checkpoint {checkpoint!r} is not None or "
-                         "'8bit'")
+def _check_cpu(op: str, x, weight, bias, checkpoint) -> None:
     if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
         raise ValueError(f"{op}: x {tuple(x.shape)} and weight "
                          f"{tuple(weight.shape)} do not fit")
     if 0 in weight.shape:
         raise ValueError(f"{op}: weight {tuple(weight.shape)} is empty")
-    if not x.is_floating_point() or (
-            x.is_cuda and x.dtype not in (torch.bfloat16, torch.float16)):
-        raise TypeError(f"{op}: {x.dtype} on {x.device.type}; bfloat16 or "
-                        "float16 on the GPU")
-    if checkpoint is not None and x.dtype == torch.float64:
+    if not x.is_floating_point():
+        raise TypeError(f"{op}: {x.dtype} is no floating type")
+    if checkpoint and x.dtype == torch.float64:
         raise TypeError(f"{op}: no 8-bit checkpoint of float64")
     for name, t in (("weight", weight), ("bias", bias)):
         if t is not None and (t.dtype != x.dtype or t.device != x.device):
@@ -148,16 +140,15 @@ def backward_cpu(dy, x, x_scales, w, pre, scales, act: int, gated: bool,
     return dx, dw, db
 
 
-class LinearFn(torch.autograd.Function):
-    """Both layers on matrices; the gated one has no residual."""
+class _LayerFn(torch.autograd.Function):
+    """Both layers on the CPU (the GPU's is in csrc/kernels/linear_ext.cc)."""
 
     @staticmethod
     def forward(ctx, x, w, b, r, act, gated, eight):
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         need = need_x or need_w or need_b
-        fwd = hip_ext().linear_forward if require_hip_for(x) else forward_cpu
-        y, pre, scales = fwd(x, w, b, r, act, gated,
-                             (2 if eight else 1) if need else 0)
+        y, pre, scales = forward_cpu(x, w, b, r, act, gated,
+                                     (2 if eight else 1) if need else 0)
         kept = x_scales = None
         if need_w:
             kept, x_scales = pack_rows(x) if eight else (x, None)
@@ -169,34 +160,44 @@ class LinearFn(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x, x_scales, w, pre, scales = ctx.saved_tensors
-        bwd = (hip_ext().linear_backward if require_hip_for(dy)
-               else backward_cpu)
         need = ctx.needs_input_grad
         dx = dw = db = None
         if any(need[:3]):
-            dx, dw, db = bwd(dy, x, x_scales, w, pre, scales, ctx.act,
-                             ctx.gated, ctx.k, *need[:3])
+            dx, dw, db = backward_cpu(dy, *ctx.saved_tensors, ctx.act,
+                                      ctx.gated, ctx.k, *need[:3])
         return dx, dw, db, dy if need[3] else None, None, None, None
 
 
-def apply(x, w, b, r, act: int, gated: bool, eight: bool) -> torch.Tensor:
-    shape = x.shape
-    n = w.shape[0] // 2 if gated else w.shape[0]
-    if len(shape) != 2:
-        x = x.reshape(shape[:-1].numel(), shape[-1])
-        if r is not None:
-            r = r.reshape(x.shape[0], n)
-    if torch.is_grad_enabled() and (
-            x.requires_grad or w.requires_grad
-            or (b is not None and b.requires_grad)
-            or (r is not None and r.requires_grad)):
-        y = LinearFn.apply(x, w, b, r, act, gated, eight)
-    elif require_hip_for(x):
-        y = hip_ext().linear_forward(x, w, b, r, act, gated, 0)[0]
-    else:
-        y = forward_cpu(x, w, b, r, act, gated, 0)[0]
-    return y if len(shape) == 2 else y.reshape(*shape[:-1], n)
+def layer(op: str, acts: dict, x, weight, bias, residual, activation,
+          checkpoint, gated: bool) -> torch.Tensor:
+    """What linear_act and gated_linear share."""
+    try:
+        act = acts[activation]
+        eight = {None: False, "8bit": True}[checkpoint]
+    except (KeyError, TypeError):
+        raise ValueError(
+            f"{op}: activation {activation!r}, checkpoint {checkpoint!r}: not "
+            f"of {list(acts)} and [None, '8bit']") from None
+    if require_hip_for(x):
+        return hip_ext().linear_layer(x, weight, bias, residual, act, gated,
+                                      eight)
+    _check_cpu(op, x, weight, bias, eight)
+    if gated and weight.shape[0] % 2:
+        raise ValueError(f"{op}: weight {tuple(weight.shape)} has no two "
+                         "halves")
+    n = weight.shape[0] // 2 if gated else weight.shape[0]
+    shape = x.shape[:-1] + (n,)
+    if residual is not None:
+        if residual.shape != shape:
+            raise ValueError(f"{op}: residual {tuple(residual.shape)}, not "
+                             f"{tuple(shape)}")
+        if residual.dtype != x.dtype or residual.device != x.device:
+            raise TypeError(f"{op}: residual is {residual.dtype} on "
+                            f"{residual.device}, x is {x.dtype} on {x.device}")
+        residual = residual.reshape(shape[:-1].numel(), n)
+    x = x.reshape(x.shape[:-1].numel(), x.shape[-1])
+    return _LayerFn.apply(x, weight, bias, residual, act, gated,
+                          eight).reshape(shape)
 
 
 def linear_act(x: torch.Tensor, weight: torch.Tensor,
@@ -211,14 +212,5 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor,
     or "silu"; ``checkpoint`` None or "8bit" (see the module).  Rows may have
     any stride; whole multiples of 8 features from 16-byte aligned rows are
     used where they lie, others are copied first.  Differentiable once."""
-    check("linear_act", x, weight, bias, activation, checkpoint, _ACTS)
-    if residual is not None:
-        want = x.shape[:-1] + weight.shape[:1]
-        if residual.shape != want:
-            raise ValueError(f"linear_act: residual {tuple(residual.shape)}, "
-                             f"not {tuple(want)}")
-        if residual.dtype != x.dtype or residual.device != x.device:
-            raise TypeError(f"linear_act: residual is {residual.dtype} on "
-                            f"{residual.device}, x is {x.dtype} on {x.device}")
-    return apply(x, weight, bias, residual, _ACTS[activation], False,
-                 checkpoint is not None)
+    return layer("linear_act", _ACTS, x, weight, bias, residual, activation,
+                 checkpoint, False)

@@ -503,13 +503,28 @@ def test_refusals():
             wrong()
 
 
-def test_second_derivatives_are_refused():
-    x = torch.randn(3, 8, requires_grad=True)
-    w = torch.randn(6, 8)
-    g, = torch.autograd.grad(linear_act(x, w, activation="gelu").sum(), x,
-                             create_graph=True)
+@pytest.mark.parametrize("device", _devices())
+def test_second_derivatives_are_refused(device):
+    t = torch.float32 if device == "cpu" else BF16
+    x = torch.randn(3, 8, device=device, dtype=t, requires_grad=True)
+    w = torch.randn(6, 8, device=device, dtype=t, requires_grad=True)
+    for leaf in (x, w):
+        g, = torch.autograd.grad(linear_act(x, w, activation="gelu").sum(),
+                                 leaf, create_graph=True)
+        with pytest.raises(RuntimeError):
+            g.sum().backward()
+
+
+@pytest.mark.parametrize("device", _devices())
+def test_changed_inputs_are_noticed(device):
+    """What the backward pass needs must not have changed since."""
+    t = torch.float32 if device == "cpu" else BF16
+    x = torch.randn(3, 8, device=device, dtype=t)
+    w = torch.randn(6, 8, device=device, dtype=t, requires_grad=True)
+    y = linear_act(x, w, activation="gelu")
+    x.zero_()
     with pytest.raises(RuntimeError):
-        g.sum().backward()
+        y.sum().backward()
 
 
 @pytest.mark.gpu
@@ -525,6 +540,29 @@ def test_refusals_on_the_gpu():
     with pytest.raises(TypeError):
         linear_act(x.half(), w.half(), residual=torch.zeros(
             4, 6, dtype=FP16))
+    x, w = x.half(), w.half()
+    b = torch.zeros(6, device="cuda").half()
+    for wrong in (
+            lambda: linear_act(x, w, activation="tanh"),
+            lambda: linear_act(x, w, checkpoint="4bit"),
+            lambda: linear_act(x, w[:, :7]),
+            lambda: linear_act(x, w[0]),
+            lambda: linear_act(x, w[:0]),
+            lambda: linear_act(x[0, 0], w),
+            lambda: linear_act(x[:, :0], w[:, :0]),
+            lambda: linear_act(x, w, b[:5]),
+            lambda: linear_act(x, w, b[None]),
+            lambda: linear_act(x, w, b, x),
+            lambda: linear_act(x, w, b, b),
+            lambda: gated_linear(x, w, activation=None),
+            lambda: gated_linear(x, w[:5]),
+            lambda: gated_linear(x, w, b[:3])):
+        with pytest.raises(ValueError):
+            wrong()
+    with pytest.raises(TypeError):
+        linear_act(x, w, b.float())
+    with pytest.raises(TypeError):
+        linear_act(x, w.bfloat16())
 
 
 # ---- on the GPU alone ----------------------------------------------------------
