@@ -12,7 +12,7 @@ MI355X-native recast (single node, 8 GPU workers + host-DRAM PS):
   POSIX shared-memory segment (/dev/shm), with per-worker gradient
   slots and seq/ack words.
 - Workers mmap the segment: gradient push is one device→host copy per
-  shard (hipMemcpyAsync once the region is hipHostRegister'ed; plain
+  shard (hipMemcpyAsync through a pinned copy of its size; plain
   copy on CPU), then a seq bump; parameter pull is one host→device
   copy. No per-tensor RPC, no serialization — the copy engine moves
   the bytes over PCIe/IF while compute streams stay busy.
@@ -658,21 +658,14 @@ class AsyncWorkerEngine:
         self._attached = True
         self.pull()
 
-    @staticmethod
-    def _pin_segment(seg: _ShmSeg, layout: _ShmLayout) -> None:
-        """hipHostRegister the mapped shard so push/pull run as true
-        pinned DMA on the copy engine (hipMemcpyAsync on a
-        side stream). Falls back to pageable copies if registration is
-        refused."""
-        try:
-            import ctypes
-            base = ctypes.addressof(ctypes.c_char.from_buffer(seg.mm))
-            r = torch.cuda.cudart().cudaHostRegister(base, layout.total, 0)
-            if int(r) != 0:
-                raise RuntimeError(f"cudaHostRegister rc={int(r)}")
-            seg.pinned = True
-        except Exception:
-            seg.pinned = False
+    def _pin_segment(self, seg: _ShmSeg, layout: _ShmLayout) -> None:
+        """A pinned copy of the shard's size, through which push and pull
+        run as true DMA on the copy engine (hipMemcpyAsync on a
+        side stream).  Allocated, not the mapping registered: a platform
+        may refuse to register memory that exists already, and the next
+        call to the GPU then reports that error as its own."""
+        seg.staging = torch.empty(layout.numel, dtype=seg.dtype,
+                                  pin_memory=True)
 
     # -- engine interface (used by Trainer) ------------------------------
     def broadcast_parameters(self, src: int = 0) -> None:
@@ -718,21 +711,19 @@ class AsyncWorkerEngine:
             if len(self._tcp) == self.num_shards:
                 return
             # mixed shm/tcp: fall through for the shm shards only
-        # push grads to every shard, bump seq (D2H straight into the
-        # shard slot — pinned DMA on the side stream when _pin_segment
-        # succeeded)
+        # push grads to every shard, bump seq (D2H into the pinned copy on
+        # the side stream, then into the shard slot)
         if self._side is not None:
             self._side.wait_stream(torch.cuda.current_stream())
             with torch.cuda.stream(self._side):
                 for s, seg in enumerate(self.segs):
                     if seg is None:
                         continue
-                    seg.grads[w].copy_(self.flat_grads[s],
-                                       non_blocking=getattr(seg, "pinned",
-                                                            False))
+                    seg.staging.copy_(self.flat_grads[s], non_blocking=True)
             self._side.synchronize()  # grads visible before the seq bump
             for s, seg in enumerate(self.segs):
                 if seg is not None:
+                    seg.grads[w].copy_(seg.staging)
                     seg.header[_ShmLayout.seq_idx(w)] = self.local_step
         else:
             for s, seg in enumerate(self.segs):
@@ -769,13 +760,13 @@ class AsyncWorkerEngine:
         for s in self._tcp:
             self._tcp_round_trip(s, push=False)
         if self._side is not None:
+            self._side.synchronize()  # the last copies out of the staging
             with torch.cuda.stream(self._side):
                 for s, seg in enumerate(self.segs):
                     if seg is None:
                         continue
-                    self.flat_params[s].copy_(seg.params,
-                                              non_blocking=getattr(
-                                                  seg, "pinned", False))
+                    seg.staging.copy_(seg.params)
+                    self.flat_params[s].copy_(seg.staging, non_blocking=True)
             torch.cuda.current_stream().wait_stream(self._side)
         else:
             for s, seg in enumerate(self.segs):
