@@ -31,6 +31,9 @@ flags.DEFINE_string("model", "resnet50", "mnist_mlp|resnet50|"
 flags.DEFINE_integer("train_steps", 100, "global steps")
 flags.DEFINE_integer("batch_size", 64, "per-worker batch size")
 flags.DEFINE_integer("seq_len", 128, "sequence length (bert)")
+flags.DEFINE_string("feed_forward", "gelu", "bert: gelu|geglu|swiglu")
+flags.DEFINE_string("act_checkpoint", "", "bert: 8bit keeps the feed-forward "
+                                          "blocks' activations in 8 bits")
 flags.DEFINE_float("learning_rate", 0.1, "base learning rate")
 flags.DEFINE_float("momentum", 0.9, "momentum (conv nets)")
 flags.DEFINE_string("checkpoint_dir", "", "chief checkpoint dir")
@@ -77,7 +80,13 @@ def main(_):
     is_chief = FLAGS.task_index == 0
     torch.manual_seed(FLAGS.seed)
     torch.backends.cudnn.benchmark = True
-    model = build_model(FLAGS.model)
+    kw = {}
+    if FLAGS.model == "bert_base":
+        kw = {"feed_forward": FLAGS.feed_forward,
+              "act_checkpoint": FLAGS.act_checkpoint or None}
+        if FLAGS.feed_forward != "gelu":
+            kw["intermediate"] = 2048  # two thirds: as many parameters
+    model = build_model(FLAGS.model, **kw)
     if torch.cuda.is_available():
         if FLAGS.dtype == "bf16":
             model = model.bfloat16()

@@ -6,16 +6,29 @@ MI355X-first: bf16 activations, fused LayerNorm HIP kernel
 (rocps.ops.layer_norm), rocBLAS/hipBLASLt GEMMs via nn.Linear, SDPA
 attention (flash path on ROCm), MLM loss through the fused
 softmax-xent kernel (vocab 30522).
+
+``feed_forward`` and ``act_checkpoint`` take the feed-forward half of every
+layer to the framework's own operators (rocps.ops.linear, rocps.ops.gated):
+
+- ``feed_forward="geglu"`` or ``"swiglu"``: a gated block,
+  ``fc2(act(x Wg^T) * (x Wu^T)) + x``; ``fc1`` then has ``2 * intermediate``
+  rows, the gate's first (two thirds of the ungated ``intermediate`` keep the
+  parameter count);
+- ``act_checkpoint="8bit"``: the block's activations are kept in 8 bits for
+  the backward pass, which halves the memory that they take.
 """
 
 from __future__ import annotations
 
+from typing import Optional
 
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from rocps.ops.gated import gated_linear
 from rocps.ops.layer_norm import LayerNorm
+from rocps.ops.linear import linear_act
 
 __all__ = ["BertModel", "bert_base"]
 
@@ -39,12 +52,26 @@ class BertSelfAttention(nn.Module):
         return self.out(o.transpose(1, 2).reshape(B, S, H))
 
 
+_GATES = {"geglu": "gelu", "swiglu": "silu"}
+
+
 class BertLayer(nn.Module):
-    def __init__(self, hidden: int, heads: int, intermediate: int):
+    def __init__(self, hidden: int, heads: int, intermediate: int,
+                 feed_forward: str = "gelu",
+                 act_checkpoint: Optional[str] = None):
         super().__init__()
+        if feed_forward != "gelu" and feed_forward not in _GATES:
+            raise ValueError(f"feed_forward {feed_forward!r} is not one of "
+                             f"{['gelu', *_GATES]}")
+        if act_checkpoint not in (None, "8bit"):
+            raise ValueError(f"act_checkpoint {act_checkpoint!r} is not None "
+                             "or '8bit'")
+        self.gate = _GATES.get(feed_forward)
+        self.act_checkpoint = act_checkpoint
         self.attn = BertSelfAttention(hidden, heads)
         self.ln1 = LayerNorm(hidden)
-        self.fc1 = nn.Linear(hidden, intermediate)
+        self.fc1 = nn.Linear(hidden, intermediate if self.gate is None
+                             else 2 * intermediate)
         self.fc2 = nn.Linear(intermediate, hidden)
         self.ln2 = LayerNorm(hidden)
 
@@ -75,21 +102,37 @@ class BertLayer(nn.Module):
                 return self.fc2(h.reshape(B, S, inter))
         return self.fc2(F.gelu(self.fc1(x), approximate="tanh"))
 
+    def _feed_forward(self, x):
+        """The block with its residual, on the framework's operators."""
+        keep = self.act_checkpoint
+        if self.gate is None:
+            h = linear_act(x, self.fc1.weight, self.fc1.bias,
+                           activation="gelu", checkpoint=keep)
+        else:
+            h = gated_linear(x, self.fc1.weight, self.fc1.bias,
+                             activation=self.gate, checkpoint=keep)
+        return linear_act(h, self.fc2.weight, self.fc2.bias, x,
+                          checkpoint=keep)
+
     def forward(self, x):
         x = self.ln1(x + self.attn(x))
-        return self.ln2(x + self._mlp(x))
+        if self.gate is None and self.act_checkpoint is None:
+            return self.ln2(x + self._mlp(x))
+        return self.ln2(self._feed_forward(x))
 
 
 class BertModel(nn.Module):
     def __init__(self, vocab: int = 30522, hidden: int = 768,
                  layers: int = 12, heads: int = 12, intermediate: int = 3072,
-                 max_pos: int = 512):
+                 max_pos: int = 512, feed_forward: str = "gelu",
+                 act_checkpoint: Optional[str] = None):
         super().__init__()
         self.tok_emb = nn.Embedding(vocab, hidden)
         self.pos_emb = nn.Embedding(max_pos, hidden)
         self.emb_ln = LayerNorm(hidden)
         self.layers = nn.ModuleList(
-            [BertLayer(hidden, heads, intermediate) for _ in range(layers)])
+            [BertLayer(hidden, heads, intermediate, feed_forward,
+                       act_checkpoint) for _ in range(layers)])
         self.mlm_dense = nn.Linear(hidden, hidden)
         self.mlm_ln = LayerNorm(hidden)
         self.mlm_out = nn.Linear(hidden, vocab)

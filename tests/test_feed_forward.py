@@ -667,3 +667,150 @@ def test_captured_training_step():
             for p, q in zip(out, step(nx, nd, keep)):
                 assert torch.equal(p, q)
         torch.cuda.synchronize()
+
+
+# ---- the operators together ------------------------------------------------------
+
+
+@pytest.mark.parametrize("device", _devices())
+@pytest.mark.parametrize("m,k,f", [(1, 64, 96), (70, 96, 200), (300, 130, 77)])
+def test_block_against_float64(m, k, f, device):
+    """A gated block with its residual, forward and backward, the second
+    layer's bounds resting on the first's."""
+    t = BF16
+    x, w1, b1, _, _ = _make(m, k, f, t, device, 20, gated=True)
+    _, w2, b2, _, dy = _make(m, f, k, t, device, 21)
+    ls = [v.detach().requires_grad_() for v in (x, w1, b1, w2, b2)]
+    h = gated_linear(*ls[:3], activation="silu")
+    y = linear_act(h, ls[3], ls[4], ls[0])
+    got = torch.autograd.grad(y, ls, dy)
+    X, W1, B1, W2, B2, D = (v.detach().cpu().double()
+                            for v in (x, w1, b1, w2, b2, dy))
+    # forward
+    P = X @ W1.t() + B1
+    ep = (k + 8) * _H * (X.abs() @ W1.abs().t() + B1.abs())
+    A, U, ea, eu = P[:, :f], P[:, f:], ep[:, :f], ep[:, f:]
+    F = _act(A, "silu")
+    Hh = F * U
+    eh = 1.13 * ea * (U.abs() + eu) + F.abs() * eu + 8 * _H * Hh.abs()
+    eh = 1.01 * (eh + _round(Hh, t))
+    Y = Hh @ W2.t() + B2 + X
+    HM = Hh.abs() + eh
+    ey = eh @ W2.abs().t() + (f + 16) * _H * (HM @ W2.abs().t() + B2.abs()
+                                              + X.abs())
+    _within(y, Y, 1.01 * (ey + _round(Y, t)), "y")
+    # backward
+    _within(got[4], D.sum(0), (m + 8) * _H * D.abs().sum(0)
+            + _round(D.sum(0), t), "db2")
+    dW2 = D.t() @ Hh
+    _within(got[3], dW2, 1.01 * (D.abs().t() @ eh + (m + 8) * _H
+                                 * (D.abs().t() @ HM) + _round(dW2, t)),
+            "dw2")
+    dH = D @ W2
+    ed = (k + 8) * _H * (D.abs() @ W2.abs())
+    ed = 1.01 * (ed + _round(dH, t))
+    sa = _slope(A, "silu")
+    es = 1.01 * (ea + 2.0 ** -16 * A.abs()) + 8 * _H   # kept in 24 bits
+    eu = 1.01 * (eu + 2.0 ** -16 * U.abs())
+    G = torch.cat([dH * U * sa, dH * F], 1)
+    DM = dH.abs() + ed
+    eg = torch.cat([
+        ed * (U * sa).abs() + DM * (eu * (sa.abs() + es) + U.abs() * es),
+        ed * F.abs() + DM * (1.13 * es + 8 * _H * F.abs())], 1)
+    eg = 1.01 * eg + 8 * _H * G.abs()
+    er = eg + 1.01 * _round(G, t)
+    GM = G.abs() + er
+    dW1 = G.t() @ X
+    _within(got[1], dW1, 1.01 * (er.t() @ X.abs() + (m + 8) * _H
+                                 * (GM.t() @ X.abs()) + _round(dW1, t)),
+            "dw1")
+    dB1 = G.sum(0)
+    _within(got[2], dB1, 1.01 * (eg.sum(0) + (m + 8) * _H * GM.sum(0)
+                                 + _round(dB1, t)), "db1")
+    # x: through the layers, rounded, plus the residual's dy, rounded
+    dX1 = G @ W1
+    e1 = er @ W1.abs() + (2 * f + 8) * _H * (GM @ W1.abs()) + _round(dX1, t)
+    _within(got[0], dX1 + D, 1.01 * (e1 + _round(dX1.abs() + D.abs(), t)),
+            "dx")
+
+
+def _bert(**kw):
+    from rocps.models.bert import bert_base
+    torch.manual_seed(3)
+    return bert_base(layers=2, hidden=64, heads=4, intermediate=96, vocab=300,
+                     max_pos=32, **kw)
+
+
+def test_bert_with_a_gated_block():
+    """The model's gradients against the same model of torch operations."""
+    import torch.nn.functional as F
+
+    from rocps.models.bert import BertLayer
+    ids = torch.randint(0, 300, (3, 16), generator=torch.Generator()
+                        .manual_seed(4))
+    for ff, act in (("geglu", lambda v: F.gelu(v, approximate="tanh")),
+                    ("swiglu", F.silu)):
+        m = _bert(feed_forward=ff)
+        assert m.layers[0].fc1.weight.shape == (192, 64)
+        m.loss(ids, ids).backward()
+        own = [p.grad.clone() for p in m.parameters()]
+        m.zero_grad()
+
+        def composed(self, x):
+            a, u = self.fc1(x).chunk(2, dim=-1)
+            return self.fc2(act(a) * u) + x
+
+        old = BertLayer._feed_forward
+        try:
+            BertLayer._feed_forward = composed
+            m.loss(ids, ids).backward()
+        finally:
+            BertLayer._feed_forward = old
+        for a, p in zip(own, m.parameters()):
+            # float32 on both sides: some hundred roundings of 2**-24
+            assert (a - p.grad).norm() <= 1e-5 * p.grad.norm() + 1e-9
+
+
+def test_bert_act_checkpoint_keeps_the_output():
+    ids = torch.randint(0, 300, (3, 16), generator=torch.Generator()
+                        .manual_seed(5))
+    for ff in ("gelu", "geglu"):
+        plain, small = _bert(feed_forward=ff), _bert(feed_forward=ff,
+                                                     act_checkpoint="8bit")
+        assert list(plain.state_dict()) == list(small.state_dict())
+        a, b = plain.loss(ids, ids), small.loss(ids, ids)
+        assert abs(a - b) <= 1e-5 * abs(a)
+        a.backward(), b.backward()
+        for p, q in zip(plain.parameters(), small.parameters()):
+            # a kept value is off by 2**-4 at most and 2**-4 / sqrt(3) in the
+            # mean square; a gradient here meets at most eight of them (two
+            # layers, two products each, an input and a slope): sqrt(8) times
+            # that is a tenth
+            assert (p.grad - q.grad).norm() <= 0.25 * p.grad.norm() + 1e-9
+    with pytest.raises(ValueError):
+        _bert(feed_forward="relu")
+    with pytest.raises(ValueError):
+        _bert(act_checkpoint="4bit")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ff", ["gelu", "geglu", "swiglu"])
+@pytest.mark.parametrize("keep", [None, "8bit"])
+def test_bert_trains_on_the_gpu(ff, keep):
+    from rocps.engine.comm import Comm
+    from rocps.engine.sync_engine import SyncEngine
+    from rocps.train.optimizer import AdamOptimizer
+    m = _bert(feed_forward=ff, act_checkpoint=keep).cuda().bfloat16()
+    before = [p.detach().clone() for p in m.layers.parameters()]
+    eng = SyncEngine(m, Comm(device=torch.device("cuda:0")))
+    opt = AdamOptimizer(1e-2)
+    ids = torch.randint(0, 300, (4, 16), device="cuda")
+    for _ in range(2):
+        eng.zero_grad()
+        opt.begin_step()
+        loss = m.loss(ids, ids)
+        eng.step(loss, opt)
+    torch.cuda.synchronize()
+    assert torch.isfinite(loss.detach())
+    for p, q in zip(before, m.layers.parameters()):
+        assert q.isfinite().all() and not torch.equal(p, q)
