@@ -65,20 +65,17 @@ struct Slope {
   long ldp;
   void* out;  // [m][ldo], zeros behind each half's n columns; or null
   long ldo;   // a multiple of 8; the gated layer's up half begins n on
-  float* sums;   // [chunks][n or 2n], or null
+  float* sums;   // [chunks][n or 2n], or null: the bias gradient's, to be
+                 // added up
   int chunks;    // rows go to this many runs
-  void* dbias;   // [n or 2n], with sums
 };
 int slope_chunks(long m, long n);
 void launch_slope(const Slope& s, hipStream_t st);
 
-// out[m][n] = sum_k A(m,k) B(n,k) in the operands' type: `a_rows` / `b_rows`
-// say that an operand lies with its rows contiguous (element (r,k) at
-// k * ld + r).  Operands 16-byte aligned with pitches of whole 16 bytes; an
-// operand by k has k in whole 16 bytes, its zeros included.
+// out[m][n] = sum_k A(m,k) B(n,k) in the operands' type.  Operands 16-byte
+// aligned with pitches of whole 16 bytes; an operand by k has k in whole 16
+// bytes, its zeros included.
 struct Matmul {
-  int type;
-  bool a_rows, b_rows;
   bool vec_out;  // n % 8 == 0, out aligned
   long m, n, k;
   const void* a;
@@ -87,15 +84,28 @@ struct Matmul {
   long ldb;
   void* out;    // [m][n]
   float* part;  // [splits][m][n], with splits > 1
-  TileChoice choice;
+  int splits;
 };
-void launch_matmul(const Matmul& p, hipStream_t st);
-// its tiles alone, to `out` or, with splits > 1, to `part`
-void matmul_tiles_bf16(const Matmul& p, hipStream_t st);
-void matmul_tiles_fp16(const Matmul& p, hipStream_t st);
-// the linear layer's, both operands by k, with splits > 1
-void split_tiles_bf16(const Matmul& p, hipStream_t st);
-void split_tiles_fp16(const Matmul& p, hipStream_t st);
+
+// The linear layer's own, both operands by k, with splits > 1.
+void split_tiles_bf16(const Matmul& p, Tile tile, hipStream_t st);
+void split_tiles_fp16(const Matmul& p, Tile tile, hipStream_t st);
+
+// dx = g W and dW = g^T x in one launch, either with m = 0 for none, and
+// after them the sums of the bias gradient's runs (see Slope).
+struct Backward {
+  int type;
+  Matmul dx;  // a = g by k, b = W by rows
+  Matmul dw;  // a = g by rows, b = x by rows
+  const float* sums;  // or null
+  int chunks;
+  long width;
+  void* dbias;
+  PairChoice choice;
+};
+void launch_backward(const Backward& b, hipStream_t st);
+void backward_tiles_bf16(const Backward& b, hipStream_t st);
+void backward_tiles_fp16(const Backward& b, hipStream_t st);
 
 // rows of `n` 16-bit values to rows of `ldo` >= n, zeros behind
 void launch_repack(const void* x, long ldx, long m, long n, void* out,

@@ -1,7 +1,7 @@
 // Backward pass of the linear and the gated layer: the gradient of the
-// pre-activations with its column sums, and the two products
+// pre-activations with its column sums, and what follows the two products
 //   dx = g W       dW = g^T x
-// on the tiled product, with no transposed copies.
+// (tile_matmul.h).
 #include "feed_forward.h"
 #include "linear.h"
 #include "tile_gemm.h"
@@ -15,7 +15,7 @@ namespace {
 // threads wide and 8 rows high.  Each value is read once and written once:
 // bound by memory.  The bias gradient's sums are taken from the fp32 values
 // before they are rounded, over rows in a fixed order (no atomics): a run's
-// sums go to `sums`, which a second kernel adds up.
+// sums go to `sums`, which blocks of the products' launch add up.
 
 // n valid values at p, zeros behind
 template <typename T>
@@ -115,25 +115,6 @@ __global__ __launch_bounds__(256) void slope_kernel(const Slope s) {
   }
 }
 
-// sums over the runs: 64 columns a block, 4 threads a column
-template <typename T>
-__global__ __launch_bounds__(256) void sums_kernel(const float* sums,
-                                                   int chunks, long width,
-                                                   T* out) {
-  __shared__ float part[4][64];
-  const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
-  const long c = (long)blockIdx.x * 64 + tx;
-  float t = 0.f;
-  if (c < width) {
-#pragma unroll 8
-    for (int r = ty; r < chunks; r += 4) t += sums[r * width + c];
-  }
-  part[ty][tx] = t;
-  __syncthreads();
-  if (ty == 0 && c < width)
-    out[c] = (T)(part[0][tx] + part[1][tx] + part[2][tx] + part[3][tx]);
-}
-
 template <typename T, bool GATED>
 void launch_slope_t(const Slope& s, hipStream_t st) {
   const dim3 grid((unsigned)((s.n + 255) / 256), s.chunks), block(256);
@@ -145,40 +126,52 @@ void launch_slope_t(const Slope& s, hipStream_t st) {
     hipLaunchKernelGGL((slope_kernel<T, kRelu, GATED>), grid, block, 0, st, s);
   else if constexpr (!GATED)
     hipLaunchKernelGGL((slope_kernel<T, kNone, GATED>), grid, block, 0, st, s);
-  if (s.sums != nullptr) {
-    const long width = GATED ? 2 * s.n : s.n;
-    hipLaunchKernelGGL((sums_kernel<T>), dim3((unsigned)((width + 63) / 64)),
-                       block, 0, st, s.sums, s.chunks, width, (T*)s.dbias);
-  }
 }
 
 // ---- splits of k -------------------------------------------------------------
 
-// sums of the splits, in their order
+// One product's sums of its splits, in their order; blocks from `first` on
+// take the other's.
+struct Join {
+  const float* part;
+  void* out;
+  long count;
+  int splits, blocks;
+};
+
 template <typename T>
-__global__ __launch_bounds__(256) void join_kernel(const float* part,
-                                                   int splits, long count,
-                                                   T* out, bool vec) {
-  const long step = (long)gridDim.x * 256 * 8;
-  for (long i = ((long)blockIdx.x * 256 + threadIdx.x) * 8; i < count;
-       i += step) {
+__global__ __launch_bounds__(256) void join_kernel(const Join a,
+                                                   const Join b) {
+  const bool one = (int)blockIdx.x < a.blocks;
+  const Join j = one ? a : b;
+  const int id = one ? blockIdx.x : blockIdx.x - a.blocks;
+  T* out = (T*)j.out;
+  const long step = (long)j.blocks * 256 * 8;
+  for (long i = ((long)id * 256 + threadIdx.x) * 8; i < j.count; i += step) {
     float v[8] = {};
-    if (vec) {
-      for (int s = 0; s < splits; s++) {
-        const tile::f32x4* p = (const tile::f32x4*)(part + s * count + i);
-        const tile::f32x4 a = p[0], b = p[1];
+    if (j.count % 8 == 0) {  // each split's begin at whole vectors
+      for (int s = 0; s < j.splits; s++) {
+        const tile::f32x4* p =
+            (const tile::f32x4*)(j.part + s * j.count + i);
+        const tile::f32x4 x = p[0], y = p[1];
 #pragma unroll
-        for (int k = 0; k < 4; k++) v[k] += a[k], v[4 + k] += b[k];
+        for (int k = 0; k < 4; k++) v[k] += x[k], v[4 + k] += y[k];
       }
       store8(out + i, v);
     } else {
-      for (int s = 0; s < splits; s++)
+      for (int s = 0; s < j.splits; s++)
 #pragma unroll
         for (int k = 0; k < 8; k++)
-          if (i + k < count) v[k] += part[s * count + i + k];
-      store_some(out + i, count - i, v);
+          if (i + k < j.count) v[k] += j.part[s * j.count + i + k];
+      store_some(out + i, j.count - i, v);
     }
   }
+}
+
+Join join_of(const Matmul& q) {
+  const long count = q.splits > 1 ? q.m * q.n : 0;
+  return {q.part, q.out, count, q.splits,
+          count == 0 ? 0 : rocps_grid_for((count + 7) / 8, 256)};
 }
 
 __global__ __launch_bounds__(256) void repack_kernel(const short* x, long ldx,
@@ -216,19 +209,16 @@ void launch_slope(const Slope& s, hipStream_t st) {
   }
 }
 
-void launch_matmul(const Matmul& q, hipStream_t st) {
-  if (q.type == 0) matmul_tiles_bf16(q, st);
-  else matmul_tiles_fp16(q, st);
-  if (q.choice.splits == 1) return;
-  const long count = q.m * q.n;
-  const dim3 grid(rocps_grid_for(count / 8, 256)), block(256);
-  const bool vec = count % 8 == 0;
+void launch_backward(const Backward& q, hipStream_t st) {
+  if (q.type == 0) backward_tiles_bf16(q, st);
+  else backward_tiles_fp16(q, st);
+  const Join a = join_of(q.dx), b = join_of(q.dw);
+  if (a.blocks + b.blocks == 0) return;
+  const dim3 grid(a.blocks + b.blocks), block(256);
   if (q.type == 0)
-    hipLaunchKernelGGL((join_kernel<__bf16>), grid, block, 0, st, q.part,
-                       q.choice.splits, count, (__bf16*)q.out, vec);
+    hipLaunchKernelGGL((join_kernel<__bf16>), grid, block, 0, st, a, b);
   else
-    hipLaunchKernelGGL((join_kernel<_Float16>), grid, block, 0, st, q.part,
-                       q.choice.splits, count, (_Float16*)q.out, vec);
+    hipLaunchKernelGGL((join_kernel<_Float16>), grid, block, 0, st, a, b);
 }
 
 void launch_repack(const void* x, long ldx, long m, long n, void* out,

@@ -228,38 +228,31 @@ std::tuple<MaybeTensor, MaybeTensor, MaybeTensor> linear_backward(
     db = at::empty({outs}, opt);
     sums = at::empty({s.chunks, outs}, f32);
     s.sums = sums.data_ptr<float>();
-    s.dbias = db->data_ptr();
   }
   if (s.out != nullptr || need_b) ff::launch_slope(s, st);
 
-  auto product = [&](ff::Matmul& q) {
-    q.type = type;
-    q.vec_out = q.n % 8 == 0;
-    q.choice = ff::choose_tile(q.m, q.n, q.k);
-    at::Tensor part;
-    if (q.choice.splits > 1) {
-      part = at::empty({q.choice.splits, q.m, q.n}, f32);
-      q.part = part.data_ptr<float>();
-    }
-    ff::launch_matmul(q, st);
-  };
-
+  // ---- the products, and the bias gradient's last sums
+  ff::Backward q{};
+  q.type = type;
+  if (need_b) {
+    q.sums = s.sums;
+    q.chunks = s.chunks;
+    q.width = outs;
+    q.dbias = db->data_ptr();
+  }
+  Rows wr, xr;
   if (need_x) {
     TORCH_CHECK(w.has_value() && w->size(0) == outs && w->size(1) == k, op,
                 ": no weight of this gradient's shape");
     check_2d(*w, dy, op, "weight");
-    const Rows wr = whole_rows(*w, st, op);
-    ff::Matmul q{};
-    q.b_rows = true;
-    q.m = m, q.n = k, q.k = outs;
-    q.a = gp, q.lda = ldg;
-    q.b = wr.p, q.ldb = wr.ld;
-    q.out = dx->data_ptr();
-    product(q);
+    wr = whole_rows(*w, st, op);
+    q.dx.m = m, q.dx.n = k, q.dx.k = outs;
+    q.dx.a = gp, q.dx.lda = ldg;
+    q.dx.b = wr.p, q.dx.ldb = wr.ld;
+    q.dx.out = dx->data_ptr();
   }
   if (need_w) {
     TORCH_CHECK(x.has_value(), op, ": no input");
-    Rows xr;
     if (x_scales.has_value()) {
       const long ldx = up_to(k, 8), ldc = up_to(k, 32);
       TORCH_CHECK(x->is_contiguous() && x->size(0) == m && x->size(1) == ldc &&
@@ -282,14 +275,25 @@ std::tuple<MaybeTensor, MaybeTensor, MaybeTensor> linear_backward(
       xr = whole_rows(*x, st, op);
     }
     dw = at::empty({outs, k}, opt);
-    ff::Matmul q{};
-    q.a_rows = q.b_rows = true;
-    q.m = outs, q.n = k, q.k = m;
-    q.a = gp, q.lda = ldg;
-    q.b = xr.p, q.ldb = xr.ld;
-    q.out = dw->data_ptr();
-    product(q);
+    q.dw.m = outs, q.dw.n = k, q.dw.k = m;
+    q.dw.a = gp, q.dw.lda = ldg;
+    q.dw.b = xr.p, q.dw.ldb = xr.ld;
+    q.dw.out = dw->data_ptr();
   }
+  const long ms[2] = {q.dx.m, q.dw.m}, ns[2] = {q.dx.n, q.dw.n},
+             ks[2] = {q.dx.k, q.dw.k};
+  q.choice = ff::choose_pair(ms, ns, ks);
+  at::Tensor parts[2];
+  for (int i = 0; i < 2; i++) {
+    ff::Matmul& p = i == 0 ? q.dx : q.dw;
+    p.vec_out = p.n % 8 == 0;
+    p.splits = q.choice.splits[i];
+    if (p.splits > 1) {
+      parts[i] = at::empty({p.splits, p.m, p.n}, f32);
+      p.part = parts[i].data_ptr<float>();
+    }
+  }
+  ff::launch_backward(q, st);
   return {dx, dw, db};
 }
 

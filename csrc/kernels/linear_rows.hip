@@ -212,15 +212,14 @@ void launch_linear_forward(const Forward& f, hipStream_t st) {
     return;
   }
   Matmul q{};
-  q.type = f.type;
   q.m = f.m, q.n = f.gated ? 2 * f.n : f.n, q.k = f.k;
   q.vec_out = q.n % 8 == 0;
   q.a = f.x, q.lda = f.ldx;
   q.b = f.w, q.ldb = f.ldw;
   q.part = f.part;
-  q.choice = f.choice;
-  if (bf) split_tiles_bf16(q, st);
-  else split_tiles_fp16(q, st);
+  q.splits = f.choice.splits;
+  if (bf) split_tiles_bf16(q, f.choice.tile, st);
+  else split_tiles_fp16(q, f.choice.tile, st);
   if (f.gated) {
     if (bf) join_forward<__bf16, true>(f, st);
     else join_forward<_Float16, true>(f, st);

@@ -31,40 +31,125 @@ struct TileChoice {
   int splits;
 };
 
-// `halves`: the gated layer's, whose tiles hold two runs of whole 32 columns.
-// `keep`: what is kept, 0 nothing, 1 pre-activations, 2 those in 8 bits.
-inline TileChoice choose_tile(long m, long n, long k, bool halves = false,
-                              int keep = 0) {
-  struct { long bm, bn; int per_cu; double alone, each, out; } const t[kTiles] =
-      {{256, 256, 1, 1.40, 1.40, 13}, {256, 128, 1, 0.80, 0.80, 15},
-       {128, 192, 1, 0.61, 0.61, 14}, {128, 128, 2, 0.50, 0.42, 9},
-       {64, 128, 2, 0.36, 0.27, 12},  {64, 64, 4, 0.34, 0.17, 8}};
-  const long cus = 256;
+struct TileCost {
+  long bm, bn;
+  int per_cu;
+  double alone, each, out;
+};
+
+inline const TileCost& tile_cost(int t) {
+  static const TileCost costs[kTiles] = {
+      {256, 256, 1, 1.40, 1.40, 13}, {256, 128, 1, 0.80, 0.80, 15},
+      {128, 192, 1, 0.61, 0.61, 14}, {128, 128, 2, 0.50, 0.42, 9},
+      {64, 128, 2, 0.36, 0.27, 12},  {64, 64, 4, 0.34, 0.17, 8}};
+  return costs[t];
+}
+
+constexpr long kCUs = 256;
+
+inline long tile_count(const TileCost& t, long m, long n) {
+  return ((m + t.bm - 1) / t.bm) * ((n + t.bn - 1) / t.bn);
+}
+
+// One product.  `halves`: the gated layer's, whose tiles hold two runs of
+// whole 32 columns; `keep`: what is kept, 0 nothing, 1 pre-activations, 2
+// those in 8 bits.
+inline TileChoice choose_tile(long m, long n, long k, bool halves, int keep) {
   const long steps = (k + 63) / 64;
   TileChoice best{k128x128, 1};
   double least = -1;
   for (int i = 0; i < kTiles; i++) {
-    if (halves && (t[i].bn == 192 || t[i].bn == 64)) continue;
-    const long tiles = ((m + t[i].bm - 1) / t[i].bm) *
-                       ((n + t[i].bn - 1) / t[i].bn);
+    const TileCost& t = tile_cost(i);
+    if (halves && (t.bn == 192 || t.bn == 64)) continue;
+    const long tiles = tile_count(t, m, n);
     const double more = keep == 0 ? 0
-                        : t[i].per_cu == 1 ? (keep == 1 ? 3 : 9)
-                                           : (keep == 1 ? 5 : 8);
-    const double out = (t[i].out + more) * t[i].bm * t[i].bn / 65536;
+                        : t.per_cu == 1 ? (keep == 1 ? 3 : 9)
+                                        : (keep == 1 ? 5 : 8);
+    const double out = (t.out + more) * t.bm * t.bn / 65536;
     for (int s = 1; s <= 16 && (s == 1 || s * 4 <= steps); s++) {
-      const long each = (tiles * s + cus - 1) / cus;  // of the fullest CU
-      const long rest = each % t[i].per_cu;
+      const long each = (tiles * s + kCUs - 1) / kCUs;  // of the fullest CU
+      const long rest = each % t.per_cu;
       double last = 0;
-      if (rest != 0)
-        last = rest * t[i].each > t[i].alone ? rest * t[i].each : t[i].alone;
-      double us = ((steps + s - 1) / s) * ((each - rest) * t[i].each + last);
+      if (rest != 0) last = rest * t.each > t.alone ? rest * t.each : t.alone;
+      double us = ((steps + s - 1) / s) * ((each - rest) * t.each + last);
       us += each * out;
       if (s > 1) us += 4 + s * 2e-6 * m * n;
       if (least < 0 || us < least) {
         least = us;
         best = {(Tile)i, s};
       }
-      if (tiles * s >= 4 * cus) break;
+      if (tiles * s >= 4 * kCUs) break;
+    }
+  }
+  return best;
+}
+
+// Two products of one launch, in tiles of one size, the longer ones first: a
+// CU that is done with its share of one goes on with the other, so what
+// counts is that all CUs end together.  A product of no rows is none.
+struct PairChoice {
+  Tile tile;
+  int splits[2];
+  bool second_first;
+};
+
+inline PairChoice choose_pair(const long m[2], const long n[2],
+                              const long k[2]) {
+  PairChoice best{k128x128, {1, 1}, false};
+  double least = -1;
+  const long steps[2] = {(k[0] + 63) / 64, (k[1] + 63) / 64};
+  for (int i = 0; i < kTiles; i++) {
+    const TileCost& t = tile_cost(i);
+    const double out = t.out * t.bm * t.bn / 65536;
+    const long tiles[2] = {tile_count(t, m[0], n[0]),
+                           tile_count(t, m[1], n[1])};
+    // splits by twos: 1, 2, 3, 4, 6, 8, 12, 16
+    static const int kSplits[8] = {1, 2, 3, 4, 6, 8, 12, 16};
+    for (int a = 0; a < 8; a++) {
+      const int s0 = kSplits[a];
+      if (a > 0 && (tiles[0] == 0 || s0 * 4 > steps[0] ||
+                    tiles[0] * s0 >= 4 * kCUs))
+        break;
+      for (int b = 0; b < 8; b++) {
+        const int s1 = kSplits[b];
+        if (b > 0 && (tiles[1] == 0 || s1 * 4 > steps[1] ||
+                      tiles[1] * s1 >= 4 * kCUs))
+          break;
+        // each block's time where every CU has its fill, and the longest's
+        const double c0 = ((steps[0] + s0 - 1) / s0) * t.each + out;
+        const double c1 = ((steps[1] + s1 - 1) / s1) * t.each + out;
+        const bool swap = tiles[0] == 0 || (tiles[1] != 0 && c1 > c0);
+        const double cl = swap ? c1 : c0, cs = swap ? c0 : c1;
+        const long nl = swap ? tiles[1] * s1 : tiles[0] * s0;
+        long ns = swap ? tiles[0] * s0 : tiles[1] * s1;
+        // the longer ones leave two classes of CUs, which the shorter fill
+        const long q = nl / kCUs, r = nl % kCUs;
+        double hi = (q + (r > 0)) * cl, lo = q * cl;
+        const long nhi = r > 0 ? r : kCUs, nlo = kCUs - nhi;
+        double end = nl > 0 ? hi : 0;
+        while (ns > 0) {
+          if (nlo > 0 && lo <= hi) {
+            lo += cs;
+            ns -= nlo;
+            end = lo > end ? lo : end;
+          } else {
+            hi += cs;
+            ns -= nhi;
+            end = hi > end ? hi : end;
+          }
+        }
+        const long most = (swap ? steps[1] + s1 - 1 : steps[0] + s0 - 1) /
+                          (swap ? s1 : s0);
+        const double lone = most * t.alone + out;
+        double us = end > lone ? end : lone;
+        if (s0 > 1 || s1 > 1) us += 4;
+        if (s0 > 1) us += s0 * 2e-6 * m[0] * n[0];
+        if (s1 > 1) us += s1 * 2e-6 * m[1] * n[1];
+        if (least < 0 || us < least) {
+          least = us;
+          best = {(Tile)i, {s0, s1}, swap};
+        }
+      }
     }
   }
   return best;

@@ -1,5 +1,6 @@
-// Plain products on the tiled kernel, with k split where there are few tiles;
-// one type's kernels, for tile_matmul_bf16.hip and tile_matmul_fp16.hip.
+// Plain products on the tiled kernel: the backward pass's two in one launch,
+// and the forward pass's with k split; one type's kernels, for
+// tile_matmul_bf16.hip and tile_matmul_fp16.hip.
 #pragma once
 
 #include "feed_forward.h"
@@ -11,34 +12,31 @@ namespace ff {
 using tile::Operand;
 using tile::Product;
 
-template <typename T, int BM, int BN, int BLOCKS, bool AROWS, bool BROWS,
-          bool SPLIT>
-__global__ __launch_bounds__(256, BLOCKS) void matmul_kernel(const Matmul q) {
+// Block `id` of a product's tiles and splits.
+template <typename T, int BM, int BN, bool AROWS, bool BROWS>
+__device__ __forceinline__ void matmul_block(char* smem, const Matmul& q,
+                                             int id) {
   using P = Product<T, BM, BN, AROWS, BROWS, false>;
-  __shared__ __attribute__((aligned(1024))) char smem[P::LDS];
   const int mt = (int)((q.m + BM - 1) / BM), nt = (int)((q.n + BN - 1) / BN);
   const int tiles = mt * nt;
-  int tm, tn, split = 0;
-  if constexpr (SPLIT) {
-    split = blockIdx.x / tiles;
-    tile::tile_of(blockIdx.x % tiles, tiles, mt, nt, tm, tn);
-  } else {
-    tile::tile_of(blockIdx.x, tiles, mt, nt, tm, tn);
-  }
+  if (id >= tiles * q.splits) return;
+  const int split = id / tiles;
+  int tm, tn;
+  tile::tile_of(id - split * tiles, tiles, mt, nt, tm, tn);
   const long m0 = (long)tm * BM, n0 = (long)tn * BN;
-  long k0 = 0, k1 = q.k;
-  if constexpr (SPLIT) {  // runs of whole steps
-    const long steps = (q.k + tile::BK - 1) / tile::BK;
-    k0 = steps * split / q.choice.splits * tile::BK;
-    k1 = steps * (split + 1) / q.choice.splits * tile::BK;
-    if (k1 > q.k) k1 = q.k;
-  }
+  // runs of whole steps
+  const long steps = (q.k + tile::BK - 1) / tile::BK;
+  const long k0 = steps * split / q.splits * tile::BK;
+  long k1 = steps * (split + 1) / q.splits * tile::BK;
+  if (k1 > q.k) k1 = q.k;
   P prod;
   prod.run(smem, Operand{q.a, q.lda, q.m}, Operand{q.b, q.ldb, q.n}, m0, n0,
            k0, k1, 0);
 
   const int lane = threadIdx.x & 63;
   const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const bool whole = q.splits == 1;
+  float* part = q.part + (long)split * q.m * q.n;
 #pragma unroll
   for (int p = 0; p < P::FN / 2; p++) {
     const long n = n0 + (wid & 1) * P::WN + p * 32 + P::column(lane);
@@ -48,61 +46,109 @@ __global__ __launch_bounds__(256, BLOCKS) void matmul_kernel(const Matmul q) {
       float v[8];
       prod.eight(i, p, v);
       if (m >= q.m || n >= q.n) continue;
-      if constexpr (SPLIT) {
-        float* o = q.part + ((long)split * q.m + m) * q.n + n;
-        if (q.vec_out) {
-          *(tile::f32x4*)o = tile::f32x4{v[0], v[1], v[2], v[3]};
-          *(tile::f32x4*)(o + 4) = tile::f32x4{v[4], v[5], v[6], v[7]};
-        } else {
-          store_some(o, q.n - n, v);
-        }
-      } else {
-        T* o = (T*)q.out + m * q.n + n;
+      const long at = m * q.n + n;
+      if (whole) {
         if (q.vec_out)
-          store8(o, v);
+          store8((T*)q.out + at, v);
         else
-          store_some(o, q.n - n, v);
+          store_some((T*)q.out + at, q.n - n, v);
+      } else if (q.vec_out) {
+        *(tile::f32x4*)(part + at) = tile::f32x4{v[0], v[1], v[2], v[3]};
+        *(tile::f32x4*)(part + at + 4) = tile::f32x4{v[4], v[5], v[6], v[7]};
+      } else {
+        store_some(part + at, q.n - n, v);
       }
     }
   }
 }
 
-template <typename T, int BM, int BN, int BLOCKS, bool AROWS, bool BROWS,
-          bool SPLIT>
-void launch_tiles(const Matmul& q, hipStream_t st) {
-  const long tiles = ((q.m + BM - 1) / BM) * ((q.n + BN - 1) / BN);
-  const int splits = SPLIT ? q.choice.splits : 1;
-  hipLaunchKernelGGL(
-      (matmul_kernel<T, BM, BN, BLOCKS, AROWS, BROWS, SPLIT>),
-      dim3((unsigned)(tiles * splits)), dim3(256), 0, st, q);
+template <typename T, int BM, int BN, int BLOCKS>
+__global__ __launch_bounds__(256, BLOCKS) void split_kernel(const Matmul q) {
+  __shared__ __attribute__((aligned(1024))) char
+      smem[Product<T, BM, BN, false, false, false>::LDS];
+  matmul_block<T, BM, BN, false, false>(smem, q, blockIdx.x);
 }
 
-template <typename T, bool AROWS, bool BROWS, bool SPLIT>
-void by_tile(const Matmul& q, hipStream_t st) {
-  switch (q.choice.tile) {
-    case k256x256:
-      return launch_tiles<T, 256, 256, 1, AROWS, BROWS, SPLIT>(q, st);
-    case k256x128:
-      return launch_tiles<T, 256, 128, 1, AROWS, BROWS, SPLIT>(q, st);
-    case k128x192:
-      return launch_tiles<T, 128, 192, 1, AROWS, BROWS, SPLIT>(q, st);
-    case k128x128:
-      return launch_tiles<T, 128, 128, 2, AROWS, BROWS, SPLIT>(q, st);
-    case k64x128:
-      return launch_tiles<T, 64, 128, 2, AROWS, BROWS, SPLIT>(q, st);
-    default:
-      return launch_tiles<T, 64, 64, 4, AROWS, BROWS, SPLIT>(q, st);
+// The bias gradient: 64 columns' sums over the runs, 4 threads a column.
+template <typename T>
+__device__ __forceinline__ void sum_block(char* smem, const Backward& b,
+                                          int id) {
+  float(*part)[64] = (float(*)[64])smem;
+  const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
+  const long c = (long)id * 64 + tx;
+  float t = 0.f;
+  if (c < b.width) {
+#pragma unroll 8
+    for (int r = ty; r < b.chunks; r += 4) t += b.sums[r * b.width + c];
+  }
+  part[ty][tx] = t;
+  __syncthreads();
+  if (ty == 0 && c < b.width)
+    ((T*)b.dbias)[c] =
+        (T)(part[0][tx] + part[1][tx] + part[2][tx] + part[3][tx]);
+}
+
+// Blocks: the longer product's, the other's, the sums'.  Each product's
+// begin at a multiple of 8, so that their numbers say the XCD.
+template <typename T, int BM, int BN, int BLOCKS>
+__global__ __launch_bounds__(256, BLOCKS)
+void backward_kernel(const Backward b, int first, int second) {
+  constexpr int LDS = Product<T, BM, BN, true, true, false>::LDS;
+  static_assert(LDS == Product<T, BM, BN, false, true, false>::LDS, "one");
+  __shared__ __attribute__((aligned(1024))) char smem[LDS];
+  const int id = blockIdx.x;
+  if (id >= first + second)
+    sum_block<T>(smem, b, id - first - second);
+  else if ((id < first) == b.choice.second_first)
+    matmul_block<T, BM, BN, true, true>(smem, b.dw,
+                                        id < first ? id : id - first);
+  else
+    matmul_block<T, BM, BN, false, true>(smem, b.dx,
+                                         id < first ? id : id - first);
+}
+
+template <typename T, int BM, int BN, int BLOCKS>
+void launch_split(const Matmul& q, hipStream_t st) {
+  const long tiles = ((q.m + BM - 1) / BM) * ((q.n + BN - 1) / BN);
+  hipLaunchKernelGGL((split_kernel<T, BM, BN, BLOCKS>),
+                     dim3((unsigned)(tiles * q.splits)), dim3(256), 0, st, q);
+}
+
+template <typename T, int BM, int BN, int BLOCKS>
+void launch_pair(const Backward& b, hipStream_t st) {
+  auto blocks = [](const Matmul& q) {
+    const long tiles = ((q.m + BM - 1) / BM) * ((q.n + BN - 1) / BN);
+    return (int)((tiles * q.splits + 7) / 8 * 8);
+  };
+  const int dx = blocks(b.dx), dw = blocks(b.dw);
+  const int first = b.choice.second_first ? dw : dx;
+  const int sums = b.sums == nullptr ? 0 : (int)((b.width + 63) / 64);
+  hipLaunchKernelGGL((backward_kernel<T, BM, BN, BLOCKS>),
+                     dim3((unsigned)(dx + dw + sums)), dim3(256), 0, st, b,
+                     first, dx + dw - first);
+}
+
+template <typename T>
+void split_tiles(const Matmul& q, Tile tile, hipStream_t st) {
+  switch (tile) {
+    case k256x256: return launch_split<T, 256, 256, 1>(q, st);
+    case k256x128: return launch_split<T, 256, 128, 1>(q, st);
+    case k128x192: return launch_split<T, 128, 192, 1>(q, st);
+    case k128x128: return launch_split<T, 128, 128, 2>(q, st);
+    case k64x128: return launch_split<T, 64, 128, 2>(q, st);
+    default: return launch_split<T, 64, 64, 4>(q, st);
   }
 }
 
 template <typename T>
-void matmul_tiles(const Matmul& q, hipStream_t st) {
-  if (q.choice.splits > 1) {
-    if (q.a_rows) by_tile<T, true, true, true>(q, st);
-    else by_tile<T, false, true, true>(q, st);
-  } else {
-    if (q.a_rows) by_tile<T, true, true, false>(q, st);
-    else by_tile<T, false, true, false>(q, st);
+void backward_tiles(const Backward& b, hipStream_t st) {
+  switch (b.choice.tile) {
+    case k256x256: return launch_pair<T, 256, 256, 1>(b, st);
+    case k256x128: return launch_pair<T, 256, 128, 1>(b, st);
+    case k128x192: return launch_pair<T, 128, 192, 1>(b, st);
+    case k128x128: return launch_pair<T, 128, 128, 2>(b, st);
+    case k64x128: return launch_pair<T, 64, 128, 2>(b, st);
+    default: return launch_pair<T, 64, 64, 4>(b, st);
   }
 }
 

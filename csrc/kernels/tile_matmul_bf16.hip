@@ -3,12 +3,12 @@
 
 namespace ff {
 
-void matmul_tiles_bf16(const Matmul& q, hipStream_t st) {
-  matmul_tiles<__bf16>(q, st);
+void backward_tiles_bf16(const Backward& b, hipStream_t st) {
+  backward_tiles<__bf16>(b, st);
 }
 
-void split_tiles_bf16(const Matmul& q, hipStream_t st) {
-  by_tile<__bf16, false, false, true>(q, st);
+void split_tiles_bf16(const Matmul& q, Tile tile, hipStream_t st) {
+  split_tiles<__bf16>(q, tile, st);
 }
 
 }  // namespace ff

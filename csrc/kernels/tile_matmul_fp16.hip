@@ -3,12 +3,12 @@
 
 namespace ff {
 
-void matmul_tiles_fp16(const Matmul& q, hipStream_t st) {
-  matmul_tiles<_Float16>(q, st);
+void backward_tiles_fp16(const Backward& b, hipStream_t st) {
+  backward_tiles<_Float16>(b, st);
 }
 
-void split_tiles_fp16(const Matmul& q, hipStream_t st) {
-  by_tile<_Float16, false, false, true>(q, st);
+void split_tiles_fp16(const Matmul& q, Tile tile, hipStream_t st) {
+  split_tiles<_Float16>(q, tile, st);
 }
 
 }  // namespace ff
