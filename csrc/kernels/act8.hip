@@ -3,8 +3,7 @@
 // A thread holds eight neighbouring values, four threads a group of 32; the
 // group's largest comes from two exchanges between neighbouring lanes.  One
 // pass over the data, 16 + 8 bytes a thread: bound by memory.
-#include "feed_forward.h"
-#include "linear.h"
+#include "unpack8.h"
 
 namespace ff {
 namespace {
@@ -28,35 +27,10 @@ __global__ __launch_bounds__(256) void pack_kernel(const Pack p) {
   }
 }
 
-template <typename T> struct Most;
-template <> struct Most<__bf16> { static constexpr float v = 3.38953139e38f; };
-template <> struct Most<_Float16> { static constexpr float v = 65504.f; };
-template <> struct Most<float> { static constexpr float v = 3.402823466e38f; };
-
 template <typename T>
 __global__ __launch_bounds__(256) void unpack_kernel(const Pack p) {
-  const long per = (p.ldx + 7) / 8, total = p.m * per;
-  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total;
-       i += (long)gridDim.x * 256) {
-    const long r = i / per, c = (i - r * per) * 8;
-    float v[8] = {};
-    if (c < p.n) {  // codes behind n, up to the multiple of 32, are zeros
-      const long at = r * p.ldc + c;
-      decode8(*(const uint2*)(p.codes + at), p.scales[at >> 5], v);
-    }
-    // The largest magnitudes may round up past the type's range: they are
-    // held at its largest value.  NaN fails both comparisons and stays.
-#pragma unroll
-    for (int k = 0; k < 8; k++) {
-      v[k] = v[k] > Most<T>::v ? Most<T>::v : v[k];
-      v[k] = v[k] < -Most<T>::v ? -Most<T>::v : v[k];
-    }
-    T* x = (T*)p.x + r * p.ldx + c;
-    if (p.vec)
-      store8(x, v);
-    else
-      store_some(x, p.ldx - c, v);
-  }
+  unpack_values<T>(p, (long)blockIdx.x * 256 + threadIdx.x,
+                   (long)gridDim.x * 256);
 }
 
 }  // namespace

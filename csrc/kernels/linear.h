@@ -49,6 +49,17 @@ void launch_linear_forward(const Forward& f, hipStream_t st);
 void forward_tiles_bf16(const Forward& f, hipStream_t st);
 void forward_tiles_fp16(const Forward& f, hipStream_t st);
 
+// Activations in 8 bits: codes [m][ldc], scales [m][ldc / 32], ldc = n to a multiple of 32
+struct Pack {
+  int type;  // 2: fp32
+  bool vec;  // 16-byte aligned rows, n in whole 16 bytes
+  long m, n;
+  void* x;
+  long ldx;
+  unsigned char* codes;
+  unsigned char* scales;
+  long ldc;
+};
 // The gradient of the pre-activations, and its sums over the rows for the
 // bias: g = dy act'(pre), or [dy u act'(g), dy act(g)] for the gated layer.
 struct Slope {
@@ -68,6 +79,8 @@ struct Slope {
   float* sums;   // [chunks][n or 2n], or null: the bias gradient's, to be
                  // added up
   int chunks;    // rows go to this many runs
+  Pack input;    // with codes: to be unpacked by the same launch
+  int strips;    // of 256 columns; launch_slope's
 };
 int slope_chunks(long m, long n);
 void launch_slope(const Slope& s, hipStream_t st);
@@ -111,17 +124,6 @@ void backward_tiles_fp16(const Backward& b, hipStream_t st);
 void launch_repack(const void* x, long ldx, long m, long n, void* out,
                    long ldo, hipStream_t st);
 
-// act8.hip; codes [m][ldc], scales [m][ldc / 32], ldc = n to a multiple of 32
-struct Pack {
-  int type;  // 2: fp32
-  bool vec;  // 16-byte aligned rows, n in whole 16 bytes
-  long m, n;
-  void* x;
-  long ldx;
-  unsigned char* codes;
-  unsigned char* scales;
-  long ldc;
-};
 void launch_pack(const Pack& p, hipStream_t st);
 void launch_unpack(const Pack& p, hipStream_t st);  // zeros to ldx behind n
 

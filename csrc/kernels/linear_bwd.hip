@@ -2,9 +2,8 @@
 // pre-activations with its column sums, and what follows the two products
 //   dx = g W       dW = g^T x
 // (tile_matmul.h).
-#include "feed_forward.h"
-#include "linear.h"
 #include "tile_gemm.h"
+#include "unpack8.h"
 
 namespace ff {
 namespace {
@@ -30,6 +29,13 @@ __device__ __forceinline__ void load_n(const T* p, long n, bool vec,
 template <typename T, int ACT, bool GATED>
 __global__ __launch_bounds__(256) void slope_kernel(const Slope s) {
   __shared__ float part[GATED ? 2 : 1][8][256];
+  if ((int)blockIdx.x >= s.strips) {
+    const long id = (long)(blockIdx.x - s.strips) * gridDim.y + blockIdx.y;
+    unpack_values<T>(
+        s.input, id * 256 + threadIdx.x,
+        (long)(gridDim.x - s.strips) * gridDim.y * 256);
+    return;
+  }
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
   const long n = (long)blockIdx.x * 256 + tx * 8;
   const long run = (s.m + s.chunks - 1) / s.chunks;
@@ -116,8 +122,18 @@ __global__ __launch_bounds__(256) void slope_kernel(const Slope s) {
 }
 
 template <typename T, bool GATED>
-void launch_slope_t(const Slope& s, hipStream_t st) {
-  const dim3 grid((unsigned)((s.n + 255) / 256), s.chunks), block(256);
+void launch_slope_t(Slope s, hipStream_t st) {
+  // without `out` and `sums` there is nothing but the input to do
+  s.strips = s.out == nullptr && s.sums == nullptr ? 0 : (s.n + 255) / 256;
+  int more = 0;
+  if (s.input.codes != nullptr) {
+    // a block for some 4096 values, 1024 blocks at least where there are so
+    // many
+    const long blocks = (s.input.m * s.input.ldx + 4095) / 4096;
+    more = (int)((blocks + s.chunks - 1) / s.chunks);
+  }
+  if (s.strips + more == 0) return;
+  const dim3 grid(s.strips + more, s.chunks), block(256);
   if (s.act == kGelu)
     hipLaunchKernelGGL((slope_kernel<T, kGelu, GATED>), grid, block, 0, st, s);
   else if (s.act == kSilu)

@@ -229,7 +229,31 @@ std::tuple<MaybeTensor, MaybeTensor, MaybeTensor> linear_backward(
     sums = at::empty({s.chunks, outs}, f32);
     s.sums = sums.data_ptr<float>();
   }
-  if (s.out != nullptr || need_b) ff::launch_slope(s, st);
+  Rows wr, xr;
+  if (need_w) {
+    TORCH_CHECK(x.has_value(), op, ": no input");
+    if (x_scales.has_value()) {
+      const long ldx = up_to(k, 8), ldc = up_to(k, 32);
+      TORCH_CHECK(x->is_contiguous() && x->size(0) == m && x->size(1) == ldc &&
+                      x->device() == dy.device(),
+                  op, ": no input of this gradient's shape");
+      xr.keep = at::empty({m, ldx}, opt);
+      ff::Pack& p = s.input;
+      p.type = type, p.vec = true;
+      p.m = m, p.n = k;
+      p.x = xr.keep.data_ptr(), p.ldx = ldx;
+      p.codes = x->data_ptr<unsigned char>();
+      p.scales = x_scales->data_ptr<unsigned char>();
+      p.ldc = ldc;
+      xr.p = p.x, xr.ld = ldx;
+    } else {
+      check_2d(*x, dy, op, "x");
+      TORCH_CHECK(x->size(0) == m && x->size(1) == k, op,
+                  ": no input of this gradient's shape");
+      xr = whole_rows(*x, st, op);
+    }
+  }
+  ff::launch_slope(s, st);
 
   // ---- the products, and the bias gradient's last sums
   ff::Backward q{};
@@ -240,7 +264,6 @@ std::tuple<MaybeTensor, MaybeTensor, MaybeTensor> linear_backward(
     q.width = outs;
     q.dbias = db->data_ptr();
   }
-  Rows wr, xr;
   if (need_x) {
     TORCH_CHECK(w.has_value() && w->size(0) == outs && w->size(1) == k, op,
                 ": no weight of this gradient's shape");
@@ -252,28 +275,6 @@ std::tuple<MaybeTensor, MaybeTensor, MaybeTensor> linear_backward(
     q.dx.out = dx->data_ptr();
   }
   if (need_w) {
-    TORCH_CHECK(x.has_value(), op, ": no input");
-    if (x_scales.has_value()) {
-      const long ldx = up_to(k, 8), ldc = up_to(k, 32);
-      TORCH_CHECK(x->is_contiguous() && x->size(0) == m && x->size(1) == ldc &&
-                      x->device() == dy.device(),
-                  op, ": no input of this gradient's shape");
-      xr.keep = at::empty({m, ldx}, opt);
-      ff::Pack p{};
-      p.type = type, p.vec = true;
-      p.m = m, p.n = k;
-      p.x = xr.keep.data_ptr(), p.ldx = ldx;
-      p.codes = x->data_ptr<unsigned char>();
-      p.scales = x_scales->data_ptr<unsigned char>();
-      p.ldc = ldc;
-      ff::launch_unpack(p, st);
-      xr.p = p.x, xr.ld = ldx;
-    } else {
-      check_2d(*x, dy, op, "x");
-      TORCH_CHECK(x->size(0) == m && x->size(1) == k, op,
-                  ": no input of this gradient's shape");
-      xr = whole_rows(*x, st, op);
-    }
     dw = at::empty({outs, k}, opt);
     q.dw.m = outs, q.dw.n = k, q.dw.k = m;
     q.dw.a = gp, q.dw.lda = ldg;
@@ -298,21 +299,29 @@ std::tuple<MaybeTensor, MaybeTensor, MaybeTensor> linear_backward(
 }
 
 static int pack_type(const at::Tensor& t, const char* op) {
+  TORCH_CHECK_TYPE(t.scalar_type() == at::kFloat ||
+                       t.scalar_type() == at::kBFloat16 ||
+                       t.scalar_type() == at::kHalf,
+                   op, ": ", t.scalar_type(),
+                   " is not bfloat16, float16 or float32");
   return t.scalar_type() == at::kFloat ? 2 : type_of(t, op);
 }
 
-// x (m, n) -> codes (m, n to a multiple of 32), scales (m, that / 32)
+// x (..., n) -> codes (rows, n to a multiple of 32), scales (rows, that / 32)
 std::tuple<at::Tensor, at::Tensor> act8_pack(at::Tensor x) {
   const char* op = "pack_activation";
-  TORCH_CHECK(x.is_cuda() && x.dim() == 2, op, ": a matrix on the GPU");
+  TORCH_CHECK(x.is_cuda(), op, ": x must be on the GPU");
+  TORCH_CHECK_VALUE(x.dim() > 0, op, ": a scalar has no last axis");
   ff::Pack p{};
   p.type = pack_type(x, op);
   c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(x.device());
-  auto v = inner_contiguous(x);
-  p.m = v.size(0), p.n = v.size(1);
+  p.m = 1, p.n = x.size(-1);
+  for (int i = 0; i + 1 < x.dim(); i++) p.m *= x.size(i);
+  auto v = inner_contiguous(x.dim() == 2 ? x : x.reshape({p.m, p.n}));
   p.ldc = up_to(p.n, 32);
-  auto codes = at::empty({p.m, p.ldc}, x.options().dtype(at::kByte));
-  auto scales = at::empty({p.m, p.ldc / 32}, x.options().dtype(at::kByte));
+  auto bytes = x.options().dtype(at::kByte).requires_grad(false);
+  auto codes = at::empty({p.m, p.ldc}, bytes);
+  auto scales = at::empty({p.m, p.ldc / 32}, bytes);
   if (codes.numel() == 0) return {codes, scales};
   p.x = v.data_ptr();
   p.ldx = p.m > 1 ? v.stride(0) : p.n;
@@ -323,27 +332,29 @@ std::tuple<at::Tensor, at::Tensor> act8_pack(at::Tensor x) {
   return {codes, scales};
 }
 
-at::Tensor act8_unpack(at::Tensor codes, at::Tensor scales, long n,
-                       at::ScalarType dtype) {
+at::Tensor act8_unpack(at::Tensor codes, at::Tensor scales,
+                       std::vector<int64_t> shape, at::ScalarType dtype) {
   const char* op = "unpack_activation";
-  TORCH_CHECK(codes.is_cuda() && codes.device() == scales.device() &&
-                  codes.scalar_type() == at::kByte &&
-                  scales.scalar_type() == at::kByte && codes.dim() == 2 &&
-                  scales.dim() == 2 && codes.is_contiguous() &&
-                  scales.is_contiguous(),
-              op, ": codes and scales as pack_activation gives them");
+  TORCH_CHECK_VALUE(codes.is_cuda() && codes.device() == scales.device() &&
+                        codes.scalar_type() == at::kByte &&
+                        scales.scalar_type() == at::kByte &&
+                        codes.dim() == 2 && scales.dim() == 2 &&
+                        codes.is_contiguous() && scales.is_contiguous() &&
+                        !shape.empty(),
+                    op, ": codes and scales as pack_activation gives them");
   ff::Pack p{};
-  p.m = codes.size(0), p.n = n, p.ldc = codes.size(1);
-  TORCH_CHECK(n >= 0 && p.ldc == up_to(n, 32) && scales.size(0) == p.m &&
-                  scales.size(1) == p.ldc / 32,
-              op, ": codes and scales as pack_activation gives them");
+  p.m = 1, p.n = shape.back(), p.ldc = up_to(p.n, 32);
+  for (size_t i = 0; i + 1 < shape.size(); i++) p.m *= shape[i];
+  TORCH_CHECK_VALUE(codes.size(0) == p.m && codes.size(1) == p.ldc &&
+                        scales.size(0) == p.m && scales.size(1) == p.ldc / 32,
+                    op, ": codes and scales as pack_activation gives them");
   c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(codes.device());
-  auto x = at::empty({p.m, n}, codes.options().dtype(dtype));
+  auto x = at::empty(shape, codes.options().dtype(dtype));
   p.type = pack_type(x, op);
   if (x.numel() == 0) return x;
   p.x = x.data_ptr();
-  p.ldx = n;
-  p.vec = n % 8 == 0;
+  p.ldx = p.n;
+  p.vec = p.n % 8 == 0;
   p.codes = codes.data_ptr<unsigned char>();
   p.scales = scales.data_ptr<unsigned char>();
   ff::launch_unpack(p, stream_of(codes));

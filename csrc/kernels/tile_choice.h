@@ -1,15 +1,16 @@
 // Which tile and how many splits of k a product of the tiled kernel takes.
 //
 // Measured on an MI355X, bf16:
-//   tile       blocks   us a step of 64 k's          us a 256 x 256 of
-//              a CU     one block    each of all the output, with all
-//                       alone        CU's at once    CUs at it
-//   256 x 256    1        1.40         1.40            13
-//   256 x 128    1        0.80         0.80            15
-//   128 x 192    1        0.61         0.61            14
-//   128 x 128    2        0.50         0.42             9
-//    64 x 128    2        0.36         0.27            12
-//    64 x  64    4        0.34         0.17             8
+//   tile       blocks   us a step of 64 k's                 us a 256 x 256
+//              a CU     one block   each of all    the same, of the output,
+//                       alone       the CU's, by   by rows   with all CUs
+//                                   k                        at it
+//   256 x 256    1        1.40         1.40         1.45        13
+//   256 x 128    1        0.80         0.80         0.86        15
+//   128 x 192    1        0.61         0.61         0.66        14
+//   128 x 128    2        0.50         0.42         0.45         9
+//    64 x 128    2        0.36         0.27         0.29        12
+//    64 x  64    4        0.34         0.17         0.25         8
 // and with pre-activations kept, 3 more where one block has the CU and 5 more
 // where they share it; in 8 bits 9 and 8 more.
 // A larger tile does more with what it reads; a smaller one leaves fewer CUs
@@ -34,14 +35,14 @@ struct TileChoice {
 struct TileCost {
   long bm, bn;
   int per_cu;
-  double alone, each, out;
+  double alone, each, rows, out;
 };
 
 inline const TileCost& tile_cost(int t) {
   static const TileCost costs[kTiles] = {
-      {256, 256, 1, 1.40, 1.40, 13}, {256, 128, 1, 0.80, 0.80, 15},
-      {128, 192, 1, 0.61, 0.61, 14}, {128, 128, 2, 0.50, 0.42, 9},
-      {64, 128, 2, 0.36, 0.27, 12},  {64, 64, 4, 0.34, 0.17, 8}};
+      {256, 256, 1, 1.40, 1.40, 1.45, 13}, {256, 128, 1, 0.80, 0.80, 0.86, 15},
+      {128, 192, 1, 0.61, 0.61, 0.66, 14}, {128, 128, 2, 0.50, 0.42, 0.45, 9},
+      {64, 128, 2, 0.36, 0.27, 0.29, 12},  {64, 64, 4, 0.34, 0.17, 0.25, 8}};
   return costs[t];
 }
 
@@ -103,7 +104,6 @@ inline PairChoice choose_pair(const long m[2], const long n[2],
     const double out = t.out * t.bm * t.bn / 65536;
     const long tiles[2] = {tile_count(t, m[0], n[0]),
                            tile_count(t, m[1], n[1])};
-    // splits by twos: 1, 2, 3, 4, 6, 8, 12, 16
     static const int kSplits[8] = {1, 2, 3, 4, 6, 8, 12, 16};
     for (int a = 0; a < 8; a++) {
       const int s0 = kSplits[a];
@@ -116,8 +116,8 @@ inline PairChoice choose_pair(const long m[2], const long n[2],
                       tiles[1] * s1 >= 4 * kCUs))
           break;
         // each block's time where every CU has its fill, and the longest's
-        const double c0 = ((steps[0] + s0 - 1) / s0) * t.each + out;
-        const double c1 = ((steps[1] + s1 - 1) / s1) * t.each + out;
+        const double c0 = ((steps[0] + s0 - 1) / s0) * t.rows + out;
+        const double c1 = ((steps[1] + s1 - 1) / s1) * t.rows + out;
         const bool swap = tiles[0] == 0 || (tiles[1] != 0 && c1 > c0);
         const double cl = swap ? c1 : c0, cs = swap ? c0 : c1;
         const long nl = swap ? tiles[1] * s1 : tiles[0] * s0;
@@ -140,7 +140,12 @@ inline PairChoice choose_pair(const long m[2], const long n[2],
         }
         const long most = (swap ? steps[1] + s1 - 1 : steps[0] + s0 - 1) /
                           (swap ? s1 : s0);
-        const double lone = most * t.alone + out;
+        // where CUs are shared, the longest block has most of one to itself
+        const long total = tiles[0] * s0 + tiles[1] * s1;
+        long share = (total + kCUs - 1) / kCUs;
+        share = share < t.per_cu ? share : t.per_cu;
+        const double with = t.rows * (1 + 0.6 * (share - 1));
+        const double lone = most * (with > t.alone ? with : t.alone) + out;
         double us = end > lone ? end : lone;
         if (s0 > 1 || s1 > 1) us += 4;
         if (s0 > 1) us += s0 * 2e-6 * m[0] * n[0];
