@@ -51,8 +51,10 @@ struct Rows {
   long ld;
 };
 
-Rows whole_rows(const at::Tensor& t, hipStream_t st, const char* op) {
-  const long m = t.size(0), n = t.size(1);
+// `n` of its columns: a copy that is one already has more.
+Rows whole_rows(const at::Tensor& t, long n, hipStream_t st, const char* op) {
+  const long m = t.size(0);
+  if (t.size(1) != n) return {t, t.data_ptr(), t.stride(0)};
   TORCH_CHECK(n < ff::kMaxPitch, op, ": a row of ", n, " is too long");
   at::Tensor u = n > 1 && t.stride(1) != 1 ? t.contiguous() : t;
   const long ld = m > 1 ? u.stride(0) : up_to(n, 8);
@@ -74,12 +76,24 @@ at::Tensor inner_contiguous(const at::Tensor& t) {
 
 }  // namespace
 
+namespace {
+
+// t has `n` columns, or is whole_rows' copy of such
+bool fits(const at::Tensor& t, long m, long n) {
+  return t.size(0) == m &&
+         (t.size(1) == n || (t.size(1) == up_to(n, 8) && t.is_contiguous()));
+}
+
+}  // namespace
+
 // keep: 0 nothing, 1 the pre-activations in their type (the gated layer's in
 // 24 bits: a byte tensor of both planes), 2 in 8 bits.  Returns y, pre or
-// codes, scales.
-std::tuple<at::Tensor, MaybeTensor, MaybeTensor> linear_forward(
+// codes, scales.  x_used and w_used, if given: what the products took, for the
+// backward pass.
+// x_used and w_used, if given: what the products took, for the backward pass.
+static std::tuple<at::Tensor, MaybeTensor, MaybeTensor> linear_forward(
     at::Tensor x, at::Tensor w, MaybeTensor bias, MaybeTensor res, long act,
-    bool gated, long keep) {
+    bool gated, long keep, at::Tensor* x_used, at::Tensor* w_used) {
   const char* op = gated ? "gated_linear" : "linear_act";
   TORCH_CHECK(x.is_cuda(), op, ": x must be on the GPU");
   ff::Forward f{};
@@ -143,7 +157,9 @@ std::tuple<at::Tensor, MaybeTensor, MaybeTensor> linear_forward(
   }
   if (m == 0) return {y, pre, scales};
   TORCH_CHECK(m < (1L << 30), op, ": ", m, " rows are too many");
-  const Rows xr = whole_rows(x, st, op), wr = whole_rows(w, st, op);
+  const Rows xr = whole_rows(x, k, st, op), wr = whole_rows(w, k, st, op);
+  if (x_used != nullptr) *x_used = xr.keep;
+  if (w_used != nullptr) *w_used = wr.keep;
   f.x = xr.p, f.ldx = xr.ld;
   f.w = wr.p, f.ldw = wr.ld;
   at::Tensor part;
@@ -161,7 +177,7 @@ std::tuple<at::Tensor, MaybeTensor, MaybeTensor> linear_forward(
 
 // The gradients of x, weight and bias, each where asked for.  x: its values,
 // or with `x_scales` their codes; pre: as linear_forward kept them.
-std::tuple<MaybeTensor, MaybeTensor, MaybeTensor> linear_backward(
+static std::tuple<MaybeTensor, MaybeTensor, MaybeTensor> linear_backward(
     at::Tensor dy, MaybeTensor x, MaybeTensor x_scales, MaybeTensor w,
     MaybeTensor pre, MaybeTensor scales, long act, bool gated, long k,
     bool need_x, bool need_w, bool need_b) {
@@ -248,9 +264,8 @@ std::tuple<MaybeTensor, MaybeTensor, MaybeTensor> linear_backward(
       xr.p = p.x, xr.ld = ldx;
     } else {
       check_2d(*x, dy, op, "x");
-      TORCH_CHECK(x->size(0) == m && x->size(1) == k, op,
-                  ": no input of this gradient's shape");
-      xr = whole_rows(*x, st, op);
+      TORCH_CHECK(fits(*x, m, k), op, ": no input of this gradient's shape");
+      xr = whole_rows(*x, k, st, op);
     }
   }
   ff::launch_slope(s, st);
@@ -265,10 +280,11 @@ std::tuple<MaybeTensor, MaybeTensor, MaybeTensor> linear_backward(
     q.dbias = db->data_ptr();
   }
   if (need_x) {
-    TORCH_CHECK(w.has_value() && w->size(0) == outs && w->size(1) == k, op,
-                ": no weight of this gradient's shape");
+    TORCH_CHECK(w.has_value(), op, ": no weight");
     check_2d(*w, dy, op, "weight");
-    wr = whole_rows(*w, st, op);
+    TORCH_CHECK(fits(*w, outs, k), op,
+                ": no weight of this gradient's shape");
+    wr = whole_rows(*w, k, st, op);
     q.dx.m = m, q.dx.n = k, q.dx.k = outs;
     q.dx.a = gp, q.dx.lda = ldg;
     q.dx.b = wr.p, q.dx.ldb = wr.ld;
@@ -379,16 +395,22 @@ struct LayerFunction : torch::autograd::Function<LayerFunction> {
                             bool gated, bool eight) {
     const bool need_x = x.requires_grad(), need_w = w.requires_grad();
     const bool need = need_x || need_w || (b && b->requires_grad());
-    auto [y, pre, scales] = linear_forward(x, w, b, r, act, gated,
-                                           need ? (eight ? 2 : 1) : 0);
-    at::Tensor kept, kept_scales;
-    if (need_w) {
-      if (eight)
-        std::tie(kept, kept_scales) = act8_pack(x);
-      else
-        kept = x;
-    }
-    ctx->save_for_backward({kept, kept_scales, need_x ? w : at::Tensor(),
+    // where rows had to be copied, the copies serve the backward pass too
+    at::Tensor kept = x, kept_scales, kept_w = w;
+    auto [y, pre, scales] =
+        linear_forward(x, w, b, r, act, gated, need ? (eight ? 2 : 1) : 0,
+                       eight ? nullptr : &kept, &kept_w);
+    if (!need_w)
+      kept = at::Tensor();
+    else if (eight)
+      std::tie(kept, kept_scales) = act8_pack(x);
+    else if (kept.size(1) == x.size(1))
+      kept = x;
+    if (!need_x)
+      kept_w = at::Tensor();
+    else if (kept_w.size(1) == w.size(1))
+      kept_w = w;
+    ctx->save_for_backward({kept, kept_scales, kept_w,
                             pre.value_or(at::Tensor()),
                             scales.value_or(at::Tensor())});
     ctx->saved_data["act"] = act;
@@ -492,14 +514,13 @@ at::Tensor linear_layer(at::Tensor x, at::Tensor w, MaybeTensor bias,
                                      grad(bias) || grad(res)))
     y = LayerFunction::apply(x, w, bias, res, (int64_t)act, gated, eight);
   else
-    y = std::get<0>(linear_forward(x, w, bias, res, act, gated, 0));
+    y = std::get<0>(
+        linear_forward(x, w, bias, res, act, gated, 0, nullptr, nullptr));
   return flat ? y : y.view(shape);
 }
 
 void bind_linear(pybind11::module& m) {
   m.def("linear_layer", &linear_layer);
-  m.def("linear_forward", &linear_forward);
-  m.def("linear_backward", &linear_backward);
   m.def("act8_pack", &act8_pack);
   m.def("act8_unpack", &act8_unpack);
 }
