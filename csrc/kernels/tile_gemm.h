@@ -26,10 +26,10 @@
 // B has two halves or more to arrive in and A one or more.  Both in the second
 // half (two of B in LDS) are 2% to 4% slower, steps of 32 in a ring of five
 // 10% to 20%: 64-byte rows cost the L2 as much as 128-byte ones.
-// 4096 x 4096 x 8192 takes 189 us with both operands by k (1458 TFLOP/s), 199
-// with B and 204 with both by rows; without the loads it would be 168, and a
-// loop of nothing but matrix instructions on random data runs at 2050 TFLOP/s
-// for the card's power.
+// 4096 x 4096 x 8192 takes 174 us with both operands by k (1582 TFLOP/s), 186
+// with B and 189 with both by rows; without the loads it was 168, and a loop of
+// nothing but matrix instructions on random data runs at 2050 TFLOP/s: the
+// card's power is the bound, the clock falls as the pipe fills.
 //
 // Loads go from memory to LDS (16 bytes a lane) without passing registers,
 // through buffer descriptors of the tile's own extent: what lies past the last
@@ -113,26 +113,49 @@ __device__ __forceinline__ long whole(long n) { return (n + 7) & ~7L; }
 //   ROWS = false  LDS [R][64]: 128 bytes a row
 //   ROWS = true   LDS [64][R]
 // PERM: rows within each 32 are permuted (by k only, see above).
+//
+// A wave fills a run of LDS, 1024 bytes a pass, so that four passes have one
+// LDS base and differ in the instruction's own offset.  That offset moves the
+// address in memory as well: `off` is so much less, and the descriptor's base
+// LEAD bytes before the operand, which no lane's offset reaches.
+constexpr int LEAD = 3 * 1024;
+
 template <int R, bool ROWS, bool PERM>
 struct Stage {
   static constexpr int BYTES = R * BK * 2;
   static constexpr int PASSES = BYTES / 4096;  // 16 bytes a thread
-  static constexpr int RPP = 32;               // by k: rows a pass
   unsigned off[PASSES];
   unsigned chunk;  // by k: this lane's 16 bytes' first k
 
-  // row0: the pass's first row, from the descriptor's base
-  __device__ __forceinline__ void init(int tid, long ld, int pass, int row0) {
-    if constexpr (ROWS) {
-      int o = pass * 4096 + tid * 16;
-      int k = o / (R * 2), b = o % (R * 2);
-      off[pass] = (unsigned)(k * ld * 2) + (b ^ swizzle(k)) + row0 * 2;
-    } else {
-      const int q = tid >> 3;
-      const int r = PERM ? ((q & 15) >> 2) * 8 + (q >> 4) * 4 + (q & 3) : q;
-      chunk = ((tid & 7) ^ swap(q)) * 8;
-      off[pass] = (unsigned)((row0 + r) * ld * 2) + chunk * 2;
+  // HALVES: two runs of R / 2 rows, which the waves take in turns; offsets
+  // count from the first row of the wave's run
+  template <bool HALVES>
+  __device__ __forceinline__ void init(int wid, int lane, long ld) {
+#pragma unroll
+    for (int p = 0; p < PASSES; p++) {
+      const int o = (wid * PASSES + p) * 1024 + lane * 16;
+      unsigned at;
+      if constexpr (ROWS) {
+        const int k = o / (R * 2), b = o % (R * 2);
+        at = (unsigned)(k * ld * 2) + (b ^ swizzle(k));
+      } else {
+        const int row = o >> 7, q = row & 31;
+        int r = (row & ~31) +
+                (PERM ? ((q & 15) >> 2) * 8 + (q >> 4) * 4 + (q & 3) : q);
+        if constexpr (HALVES) r = (wid >> 1) * (R / 4) + r % (R / 4);
+        chunk = ((lane & 7) ^ swap(row)) * 8;
+        at = (unsigned)(r * ld * 2) + chunk * 2;
+      }
+      off[p] = at + LEAD - (p & 3) * 1024;
     }
+  }
+
+  // The last k's: lanes past them load nothing.  Once is enough for a step;
+  // from then on they stay past.
+  __device__ __forceinline__ void cut(int left) {
+#pragma unroll
+    for (int p = 0; p < PASSES; p++)
+      off[p] = (int)chunk < left ? off[p] : PAST;
   }
 
   // By k: eight lanes read the same 16 bytes of eight rows, of which two fill
@@ -153,10 +176,10 @@ struct Stage {
 // gives zeros), raw 32-bit data.
 using Descriptor = __attribute__((ext_vector_type(4))) int;
 
-__device__ __forceinline__ Descriptor descriptor(const void* p, long bytes) {
-  const unsigned long a = (unsigned long)p;
-  return Descriptor{(int)(unsigned)a, (int)((a >> 32) & 0xffff),
-                    bytes < 0 ? 0 : (int)bytes, 0x00020000};
+__device__ __forceinline__ Descriptor descriptor(const char* p, int bytes) {
+  const unsigned long a = (unsigned long)(p - LEAD);
+  return Descriptor{(int)(unsigned)a, (int)((a >> 32) & 0xffff), bytes,
+                    0x00020000};
 }
 
 // Waits for all loads to LDS (LOADS > 0: but the last so many) and, if READS,
@@ -176,18 +199,37 @@ __device__ __forceinline__ void barrier() {
   asm volatile("" ::: "memory");
 }
 
-// 16 bytes a lane from memory to LDS at `dst` + 16 lane; `dst` is the wave's.
-// As an instruction, because before a transposing read of LDS the compiler
-// waits for every such load that it knows of.  It has no register to write,
-// and `wait` is what waits for it.  M0, which it takes the place from, is the
-// compiler's only around instructions that these kernels do not have.
-__device__ __forceinline__ void load_lds(Descriptor r, lds_char* dst,
-                                         unsigned off, int soff) {
-  asm volatile(
-      "s_mov_b32 m0, %0\n\ts_nop 0\n\t"
-      "buffer_load_dwordx4 %1, %2, %3 offen lds"
-      :
-      : "s"((unsigned)(unsigned long)dst), "v"(off), "s"(r), "s"(soff));
+// 16 bytes a lane from memory to LDS at M0 + 1024 PASS + 16 lane.  As an
+// instruction, because before a transposing read of LDS the compiler waits for
+// every such load that it knows of.  It has no register to write, and `wait`
+// is what waits for it.  M0 is the compiler's only around instructions that
+// these kernels do not have; one other instruction has to lie between `set_m0`
+// and the load.  As every instruction between two matrix instructions counts
+// (one idle one more to each load costs 2% to 8%), M0 is set for four loads
+// and their lanes' offsets are ready.
+__device__ __forceinline__ void set_m0(lds_char* dst) {
+  asm volatile("s_mov_b32 m0, %0" : : "s"((unsigned)(unsigned long)dst));
+}
+
+__device__ __forceinline__ void load_lds(Descriptor r, unsigned off, int soff,
+                                         int pass) {
+  switch (pass & 3) {
+    case 0:
+      asm volatile("buffer_load_dwordx4 %0, %1, %2 offen lds"
+                   : : "v"(off), "s"(r), "s"(soff));
+      break;
+    case 1:
+      asm volatile("buffer_load_dwordx4 %0, %1, %2 offen offset:1024 lds"
+                   : : "v"(off), "s"(r), "s"(soff));
+      break;
+    case 2:
+      asm volatile("buffer_load_dwordx4 %0, %1, %2 offen offset:2048 lds"
+                   : : "v"(off), "s"(r), "s"(soff));
+      break;
+    default:
+      asm volatile("buffer_load_dwordx4 %0, %1, %2 offen offset:3072 lds"
+                   : : "v"(off), "s"(r), "s"(soff));
+  }
 }
 
 // Blocks go round the 8 XCDs by their number; giving each XCD a run of
@@ -219,7 +261,7 @@ struct Product {
   using SA = Stage<BM, AROWS, false>;
   using SB = Stage<BN, BROWS, true>;
   static constexpr int LDS = 2 * SA::BYTES + 3 * SB::BYTES;
-  static_assert(!SPLITB || (!BROWS && WN / 2 >= SB::RPP), "whole passes");
+  static_assert(!SPLITB || !BROWS, "the weights lie by k");
 
   f32x4 acc[FM][FN];
 
@@ -248,40 +290,46 @@ struct Product {
 
   // The loads of one operand, a step at a time.  By k the descriptor stays and
   // k is the loads' scalar offset: rows are told apart by the lanes' offsets
-  // alone, k's by `in`.  By rows the descriptor moves on, over what is left.
-  template <bool ROWS>
+  // alone, k's by `cut`.  By rows the descriptor moves on, over a step's k's.
+  template <typename S, bool ROWS>
   struct Feed {
     const char* p;
-    long rest;  // bytes from p
-    long step;  // bytes a step
-    int k;      // bytes
+    long step;             // bytes a step
+    int full, part, soff;  // a step's extent, the last step's
+    int left;              // k's from this step on
+    Descriptor d;
 
     __device__ __forceinline__ void init(const Operand& o, long r0, int rows,
                                          long k0, long k1) {
-      const long left = o.rows - r0;
+      const long ext = whole(o.rows - r0);
+      left = (int)(k1 - k0);
+      soff = 0;
       if constexpr (ROWS) {
         p = (const char*)o.p + (k0 * o.ld + r0) * 2;
-        rest = ((k1 - k0 - 1) * o.ld + whole(left)) * 2;
         step = BK * o.ld * 2;
+        full = (int)(((BK - 1) * o.ld + ext) * 2) + LEAD;
+        part = (int)((((left - 1) % BK) * o.ld + ext) * 2) + LEAD;
       } else {
+        const long has = o.rows - r0;
         p = (const char*)o.p + (r0 * o.ld + k0) * 2;
-        rest = (((left < rows ? left : rows) - 1) * o.ld + whole(k1 - k0)) * 2;
-        step = BK * 2;
+        const long bytes =
+            (((has < rows ? has : rows) - 1) * o.ld + whole(left)) * 2 + LEAD;
+        // rows past the last: no extent
+        d = descriptor(p, has > 0 ? (int)bytes : 0);
       }
-      k = 0;
     }
-    __device__ __forceinline__ Descriptor get() const {
-      // an extent past 2^31 - 1 is as good as that: a step's offsets are less
-      const long most = 0x7fffffffL;
-      return descriptor(p, rest > most ? most : rest);
+    // to be called before a step's loads
+    __device__ __forceinline__ void begin(S& s) {
+      if constexpr (ROWS) {
+        d = descriptor(p, left >= BK ? full : left > 0 ? part : 0);
+      } else {
+        if (left < BK) s.cut(left);
+      }
     }
     __device__ __forceinline__ void next() {
-      if constexpr (ROWS) {
-        p += step;
-        rest -= step;
-      } else {
-        k += BK * 2;
-      }
+      left -= BK;
+      if constexpr (ROWS) p += step;
+      else soff += BK * 2;
     }
   };
 
@@ -296,64 +344,36 @@ struct Product {
 
     SA sa;
     SB sb;
-#pragma unroll
-    for (int p = 0; p < SA::PASSES; p++) sa.init(tid, A.ld, p, AROWS ? 0 : p * SA::RPP);
-#pragma unroll
-    for (int p = 0; p < SB::PASSES; p++) {
-      int r = p * SB::RPP;
-      if constexpr (SPLITB) r = (r / WN) * (WN / 2) + r % (WN / 2);
-      sb.init(tid, B.ld, p, BROWS ? 0 : r);
-    }
-
-    Feed<AROWS> fa;
-    Feed<BROWS> fb, fb2;
-    constexpr int RB = SPLITB ? BN / 2 : BN;
+    sa.template init<false>(wid, lane, A.ld);
+    sb.template init<SPLITB>(wid, lane, B.ld);
+    Feed<SA, AROWS> fa;
+    Feed<SB, BROWS> fb;
     fa.init(A, m0, BM, k0, k1);
-    fb.init(B, n0, RB, k0, k1);
-    if constexpr (SPLITB) {
-      fb2 = fb;
-      fb2.p += second * B.ld * 2;
+    {
+      // of two runs, odd waves take the second
+      Operand o = B;
+      if (SPLITB && (wid & 1)) o.p = (const char*)B.p + second * B.ld * 2;
+      fb.init(o, n0, SPLITB ? BN / 2 : BN, k0, k1);
     }
     const int steps = (int)((k1 - k0 + BK - 1) / BK);
-    const int extent = (int)(k1 - k0);
-    int ka = 0, kb = 0;  // the next loads' first k
     lds_char* const ldsa = smem;
     lds_char* const ldsb = smem + 2 * SA::BYTES;
 
-    // One operand's loads of its next step, some at a time.  Past the last
-    // step all lanes' offsets lie outside: zeros, which nothing reads.
-    struct Source {
-      Descriptor r, r2;
-      bool in;
+    // Load p of an operand's step, into the buffer `to`; M0 is set for four
+    // of them, one matrix instruction (or an idle one) before.
+    auto base_a = [&](lds_char* to, int p) {
+      set_m0(to + wid * (SA::PASSES * 1024) + (p & ~3) * 1024);
     };
-    auto source_a = [&]() {
-      Source s;
-      s.r = fa.get();
-      s.in = AROWS || (int)sa.chunk < extent - ka;
-      return s;
+    auto base_b = [&](lds_char* to, int p) {
+      set_m0(to + wid * (SB::PASSES * 1024) + (p & ~3) * 1024);
     };
-    auto source_b = [&]() {
-      Source s;
-      s.r = fb.get();
-      if constexpr (SPLITB) s.r2 = fb2.get();
-      s.in = BROWS || (int)sb.chunk < extent - kb;
-      return s;
+    auto load_a = [&](int p) {
+      load_lds(fa.d, sa.off[p], fa.soff, p);
+      if (p == SA::PASSES - 1) fa.next();
     };
-    auto load_a = [&](const Source& s, lds_char* to, int p) {
-      load_lds(s.r, to + wid * 1024 + p * 4096, s.in ? sa.off[p] : PAST, fa.k);
-      if (p == SA::PASSES - 1) {
-        fa.next();
-        ka += BK;
-      }
-    };
-    auto load_b = [&](const Source& s, lds_char* to, int p) {
-      const bool up = SPLITB && (p * SB::RPP) % WN >= WN / 2;
-      load_lds(up ? s.r2 : s.r, to + wid * 1024 + p * 4096,
-               s.in ? sb.off[p] : PAST, fb.k);
-      if (p == SB::PASSES - 1) {
-        fb.next();
-        kb += BK;
-      }
+    auto load_b = [&](int p) {
+      load_lds(fb.d, sb.off[p], fb.soff, p);
+      if (p == SB::PASSES - 1) fb.next();
     };
 
     // ---- fragment addresses --------------------------------------------
@@ -408,7 +428,13 @@ struct Product {
                     i16x8(&na)[FM], i16x8(&nb)[FN], lds_char* ra,
                     lds_char* rb, int kk, bool b_loads, lds_char* to) {
       const int loads = b_loads ? SB::PASSES : SA::PASSES;
-      const Source src = b_loads ? source_b() : source_a();
+      if (b_loads) {
+        fb.begin(sb);
+        base_b(to, 0);
+      } else {
+        fa.begin(sa);
+        base_a(to, 0);
+      }
 #pragma unroll
       for (int i = 0; i < FM; i++)
 #pragma unroll
@@ -429,10 +455,13 @@ struct Product {
 #pragma unroll
           for (int q = slot * loads / SLOTS; q < (slot + 1) * loads / SLOTS;
                q++) {
-            if (b_loads)
-              load_b(src, to, q);
-            else
-              load_a(src, to, q);
+            if (b_loads) {
+              load_b(q);
+              if ((q & 3) == 3 && q + 1 < loads) base_b(to, q + 1);
+            } else {
+              load_a(q);
+              if ((q & 3) == 3 && q + 1 < loads) base_a(to, q + 1);
+            }
           }
           __builtin_amdgcn_sched_barrier(0);
         }
@@ -446,14 +475,24 @@ struct Product {
     i16x8 a0[FM], b0[FN], a1[FM], b1[FN];
 #pragma unroll
     for (int n = 0; n < 2; n++) {
-      const Source rb = source_b();
+      fb.begin(sb);
 #pragma unroll
-      for (int p = 0; p < SB::PASSES; p++)
-        load_b(rb, ldsb + n * SB::BYTES, p);
-      const Source ra = source_a();
+      for (int p = 0; p < SB::PASSES; p++) {
+        if ((p & 3) == 0) {
+          base_b(ldsb + n * SB::BYTES, p);
+          asm volatile("s_nop 0");
+        }
+        load_b(p);
+      }
+      fa.begin(sa);
 #pragma unroll
-      for (int p = 0; p < SA::PASSES; p++)
-        load_a(ra, ldsa + n * SA::BYTES, p);
+      for (int p = 0; p < SA::PASSES; p++) {
+        if ((p & 3) == 0) {
+          base_a(ldsa + n * SA::BYTES, p);
+          asm volatile("s_nop 0");
+        }
+        load_a(p);
+      }
     }
     wait<SA::PASSES + SB::PASSES, false>();  // step 0 has landed
     barrier();
