@@ -74,36 +74,39 @@ def _unpack_cpu(codes, scales, n: int, dtype: torch.dtype) -> torch.Tensor:
 
 
 def pack_rows(x: torch.Tensor):
-    """(rows, n) -> codes, scales."""
+    """(..., n) -> codes, scales."""
     if require_hip_for(x):
         return hip_ext().act8_pack(x)
-    return _pack_cpu(x)
+    if x.dtype not in _TYPES:
+        raise TypeError(f"pack_activation: {x.dtype} is not one of {_TYPES}")
+    if x.dim() == 0:
+        raise ValueError("pack_activation: a scalar has no last axis")
+    return _pack_cpu(x.detach().reshape(x.shape[:-1].numel(), x.shape[-1]))
 
 
-def unpack_rows(codes, scales, n: int, dtype: torch.dtype) -> torch.Tensor:
+def unpack_rows(codes, scales, shape, dtype: torch.dtype) -> torch.Tensor:
     if require_hip_for(codes):
-        return hip_ext().act8_unpack(codes, scales, n, dtype)
-    return _unpack_cpu(codes, scales, n, dtype)
+        return hip_ext().act8_unpack(codes, scales, shape, dtype)
+    if dtype not in _TYPES:
+        raise TypeError(f"unpack_activation: {dtype} is not one of {_TYPES}")
+    n = shape[-1]
+    if (codes.shape != (shape[:-1].numel(), (n + 31) // 32 * 32)
+            or scales.shape != (codes.shape[0], codes.shape[1] // 32)):
+        raise ValueError("unpack_activation: codes and scales as "
+                         "pack_activation gives them")
+    return _unpack_cpu(codes, scales, n, dtype).reshape(shape)
 
 
 def pack_activation(x: torch.Tensor) -> PackedActivation:
     """``x`` (any shape but a scalar's; bfloat16, float16 or float32) in 8
     bits, in groups of 32 along its last axis.  Nothing is differentiated
     through it: the values are those of ``x.detach()``."""
-    if x.dtype not in _TYPES:
-        raise TypeError(f"pack_activation: {x.dtype} is not one of {_TYPES}")
-    if x.dim() == 0:
-        raise ValueError("pack_activation: a scalar has no last axis")
-    rows = x.detach().reshape(x.shape[:-1].numel(), x.shape[-1])
-    codes, scales = pack_rows(rows)
+    codes, scales = pack_rows(x)
     return PackedActivation(codes, scales, x.shape, x.dtype)
 
 
 def unpack_activation(packed: PackedActivation,
                       dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """The values that ``packed`` holds, in their own type or in ``dtype``."""
-    dtype = packed.dtype if dtype is None else dtype
-    if dtype not in _TYPES:
-        raise TypeError(f"unpack_activation: {dtype} is not one of {_TYPES}")
-    return unpack_rows(packed.codes, packed.scales, packed.shape[-1],
-                       dtype).reshape(packed.shape)
+    codes, scales, shape, own = packed
+    return unpack_rows(codes, scales, shape, own if dtype is None else dtype)

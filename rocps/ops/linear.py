@@ -119,10 +119,11 @@ def backward_cpu(dy, x, x_scales, w, pre, scales, act: int, gated: bool,
             c, s = pre.shape[1] // 2, scales.shape[1] // 2
             pre = torch.cat(
                 [unpack_rows(pre[:, a * c:(a + 1) * c].contiguous(),
-                             scales[:, a * s:(a + 1) * s].contiguous(), n,
+                             scales[:, a * s:(a + 1) * s].contiguous(),
+                             dy.shape,
                              torch.float32) for a in (0, 1)], 1)
         else:
-            pre = unpack_rows(pre, scales, n, torch.float32)
+            pre = unpack_rows(pre, scales, dy.shape, torch.float32)
         if gated:
             a, u = pre[:, :n], pre[:, n:]
             g = torch.cat([d * u * slope_cpu(a, act), d * act_cpu(a, act)], 1)
@@ -133,7 +134,8 @@ def backward_cpu(dy, x, x_scales, w, pre, scales, act: int, gated: bool,
         dx = (g @ wide(w)).to(dy.dtype)
     if need_w:
         if x_scales is not None:
-            x = unpack_rows(x, x_scales, k, dy.dtype)
+            x = unpack_rows(x, x_scales, torch.Size((dy.shape[0], k)),
+                            dy.dtype)
         dw = (g.t() @ wide(x)).to(dy.dtype)
     if need_b:
         db = g.sum(0).to(dy.dtype)
