@@ -179,18 +179,41 @@ __device__ __forceinline__ void store8(T* p, const float* v) {
   *(Vec8<T>*)p = u;
 }
 
-// n valid values from an address of any alignment, zeros behind them
+// n valid values from an address of any alignment, zeros behind them.  Eight
+// are one access all the same, which the memory's units split where they have
+// to: rows of odd lengths cost little more than others.
+template <typename T>
+using Any8 __attribute__((aligned(sizeof(T)))) = Vec8<T>;
+
+template <typename T>
+__device__ __forceinline__ Vec8<T> some8(const T* p, long n) {
+  if (n >= 8) return *(const Any8<T>*)p;
+  Vec8<T> u = {};
+#pragma unroll
+  for (int k = 0; k < 8; k++)
+    if (k < n) u[k] = p[k];
+  return u;
+}
+
 template <typename T>
 __device__ __forceinline__ void load_some(const T* p, long n, float* v) {
+  const Vec8<T> u = some8(p, n);
 #pragma unroll
-  for (int k = 0; k < 8; k++) v[k] = k < n ? (float)p[k] : 0.f;
+  for (int k = 0; k < 8; k++) v[k] = (float)u[k];
 }
 
 template <typename T>
 __device__ __forceinline__ void store_some(T* p, long n, const float* v) {
+  Vec8<T> u;
 #pragma unroll
-  for (int k = 0; k < 8; k++)
-    if (k < n) p[k] = (T)v[k];
+  for (int k = 0; k < 8; k++) u[k] = (T)v[k];
+  if (n >= 8) {
+    *(Any8<T>*)p = u;
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; k++)
+      if (k < n) p[k] = u[k];
+  }
 }
 
 __device__ __forceinline__ void store24(unsigned short* hi, unsigned char* lo,

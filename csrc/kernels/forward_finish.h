@@ -72,13 +72,7 @@ __device__ __forceinline__ Vec8<T> residual8(const Forward& f, long m, long n) {
   Vec8<T> r = {};
   if (f.res != nullptr && m < f.m && n < f.n) {
     const T* p = (const T*)f.res + m * f.ldr + n;
-    if (f.vec_out) {
-      r = *(const Vec8<T>*)p;
-    } else {
-#pragma unroll
-      for (int k = 0; k < 8; k++)
-        if (n + k < f.n) r[k] = p[k];
-    }
+    r = f.vec_out ? *(const Vec8<T>*)p : some8(p, f.n - n);
   }
   return r;
 }

@@ -14,7 +14,8 @@ constexpr long kMaxPitch = 1L << 22;
 
 // y = act(x W^T + bias) + residual; with `gated`, W = [Wg; Wu] of 2n rows and
 // y = act(x Wg^T + bias[:n]) * (x Wu^T + bias[n:]).
-// x and w: 16-byte aligned, pitch and k in whole 16 bytes.
+// x and w: 16-byte aligned with pitches of whole 16 bytes and zeros behind k up
+// to such.
 struct Forward {
   int type, act;
   bool gated;
@@ -49,7 +50,8 @@ void launch_linear_forward(const Forward& f, hipStream_t st);
 void forward_tiles_bf16(const Forward& f, hipStream_t st);
 void forward_tiles_fp16(const Forward& f, hipStream_t st);
 
-// Activations in 8 bits: codes [m][ldc], scales [m][ldc / 32], ldc = n to a multiple of 32
+// Activations in 8 bits: codes [m][ldc], scales [m][ldc / 32], ldc = n to a
+// multiple of 32
 struct Pack {
   int type;  // 2: fp32
   bool vec;  // 16-byte aligned rows, n in whole 16 bytes

@@ -74,9 +74,12 @@ at::Tensor inner_contiguous(const at::Tensor& t) {
   return t.size(1) > 1 && t.stride(1) != 1 ? t.contiguous() : t;
 }
 
-}  // namespace
-
-namespace {
+// A launch that was refused (more blocks than a grid can have, say) has written
+// nothing.
+void check_launch(const char* op) {
+  const hipError_t e = hipGetLastError();
+  TORCH_CHECK(e == hipSuccess, op, ": ", hipGetErrorString(e));
+}
 
 // t has `n` columns, or is whole_rows' copy of such
 bool fits(const at::Tensor& t, long m, long n) {
@@ -90,7 +93,6 @@ bool fits(const at::Tensor& t, long m, long n) {
 // 24 bits: a byte tensor of both planes), 2 in 8 bits.  Returns y, pre or
 // codes, scales.  x_used and w_used, if given: what the products took, for the
 // backward pass.
-// x_used and w_used, if given: what the products took, for the backward pass.
 static std::tuple<at::Tensor, MaybeTensor, MaybeTensor> linear_forward(
     at::Tensor x, at::Tensor w, MaybeTensor bias, MaybeTensor res, long act,
     bool gated, long keep, at::Tensor* x_used, at::Tensor* w_used) {
@@ -172,6 +174,7 @@ static std::tuple<at::Tensor, MaybeTensor, MaybeTensor> linear_forward(
     }
   }
   ff::launch_linear_forward(f, st);
+  check_launch(op);
   return {y, pre, scales};
 }
 
@@ -311,6 +314,7 @@ static std::tuple<MaybeTensor, MaybeTensor, MaybeTensor> linear_backward(
     }
   }
   ff::launch_backward(q, st);
+  check_launch(op);
   return {dx, dw, db};
 }
 
@@ -345,6 +349,7 @@ std::tuple<at::Tensor, at::Tensor> act8_pack(at::Tensor x) {
   p.codes = codes.data_ptr<unsigned char>();
   p.scales = scales.data_ptr<unsigned char>();
   ff::launch_pack(p, stream_of(x));
+  check_launch(op);
   return {codes, scales};
 }
 
@@ -374,6 +379,7 @@ at::Tensor act8_unpack(at::Tensor codes, at::Tensor scales,
   p.codes = codes.data_ptr<unsigned char>();
   p.scales = scales.data_ptr<unsigned char>();
   ff::launch_unpack(p, stream_of(codes));
+  check_launch(op);
   return x;
 }
 

@@ -21,7 +21,9 @@ using tile::i16x8;
 // launch, so a single token costs what its weights do: 4096 -> 2 x 8192 takes
 // 29.9 us (4.5 TB/s), 4096 -> 4096 8.1 us, 16 rows of that 10.8, 32 rows 13.8.
 // From there on x's loads are more than the weights': 40 rows take 17.6 us,
-// the tiled product with k split six times 14.9 (and 14.3 for 32).
+// the tiled product with k split six times 14.9 (and 14.3 for 32).  Rows of odd
+// lengths are copied first: read as they lie, 16 bytes at any address, 24 rows
+// of 4095 -> 4095 take 39 us, with the copy of the weights 34.
 constexpr int kWaves = 8, kTurns = 4;
 
 template <typename T, int MF, bool GATED, int KEEP>
@@ -133,7 +135,6 @@ template <typename T, bool GATED, int KEEP>
 __global__ __launch_bounds__(256) void join_forward_kernel(const Forward f) {
   const long per = (f.n + 31) / 32 * 4, total = f.m * per;
   const long width = GATED ? 2 * f.n : f.n;
-  const bool vec = f.n % 8 == 0;
   for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total;
        i += (long)gridDim.x * 256) {
     const long m = i / per, n = (i - m * per) * 8;
@@ -144,25 +145,14 @@ __global__ __launch_bounds__(256) void join_forward_kernel(const Forward f) {
     if constexpr (!GATED) r = residual8<T>(f, m, n);
     for (int s = 0; s < f.choice.splits; s++) {
       const float* p = f.part + ((long)s * f.m + m) * width + n;
-      if (vec && n < f.n) {
+      float a[8];
+      load_some(p, f.n - n, a);
 #pragma unroll
-        for (int q = 0; q < 2; q++) {
-          const f32x4 a = ((const f32x4*)p)[q];
+      for (int k = 0; k < 8; k++) v[k] += a[k];
+      if constexpr (GATED) {
+        load_some(p + f.n, f.n - n, a);
 #pragma unroll
-          for (int r = 0; r < 4; r++) v[q * 4 + r] += a[r];
-          if constexpr (GATED) {
-            const f32x4 b = ((const f32x4*)(p + f.n))[q];
-#pragma unroll
-            for (int r = 0; r < 4; r++) u[q * 4 + r] += b[r];
-          }
-        }
-      } else {
-#pragma unroll
-        for (int k = 0; k < 8; k++)
-          if (n + k < f.n) {
-            v[k] += p[k];
-            if constexpr (GATED) u[k] += p[f.n + k];
-          }
+        for (int k = 0; k < 8; k++) u[k] += a[k];
       }
     }
     finish8<T, KEEP, -1, GATED, 1, 2>(f, m, n, true, v, u, r);

@@ -83,7 +83,6 @@ __device__ __forceinline__ void mfma(f32x4& c, i16x8 b, i16x8 a) {
   }
 }
 
-
 // the same as a value, for the compiler to schedule
 template <typename T>
 __device__ __forceinline__ f32x4 mfma_value(i16x8 b, i16x8 a, f32x4 c) {
@@ -211,24 +210,20 @@ __device__ __forceinline__ void set_m0(lds_char* dst) {
   asm volatile("s_mov_b32 m0, %0" : : "s"((unsigned)(unsigned long)dst));
 }
 
+template <int AT>
+__device__ __forceinline__ void load_lds_at(Descriptor r, unsigned off,
+                                            int soff) {
+  asm volatile("buffer_load_dwordx4 %0, %1, %2 offen offset:%3 lds"
+               : : "v"(off), "s"(r), "s"(soff), "n"(AT));
+}
+
 __device__ __forceinline__ void load_lds(Descriptor r, unsigned off, int soff,
                                          int pass) {
   switch (pass & 3) {
-    case 0:
-      asm volatile("buffer_load_dwordx4 %0, %1, %2 offen lds"
-                   : : "v"(off), "s"(r), "s"(soff));
-      break;
-    case 1:
-      asm volatile("buffer_load_dwordx4 %0, %1, %2 offen offset:1024 lds"
-                   : : "v"(off), "s"(r), "s"(soff));
-      break;
-    case 2:
-      asm volatile("buffer_load_dwordx4 %0, %1, %2 offen offset:2048 lds"
-                   : : "v"(off), "s"(r), "s"(soff));
-      break;
-    default:
-      asm volatile("buffer_load_dwordx4 %0, %1, %2 offen offset:3072 lds"
-                   : : "v"(off), "s"(r), "s"(soff));
+    case 0: return load_lds_at<0>(r, off, soff);
+    case 1: return load_lds_at<1024>(r, off, soff);
+    case 2: return load_lds_at<2 * 1024>(r, off, soff);
+    default: return load_lds_at<3 * 1024>(r, off, soff);
   }
 }
 
@@ -254,7 +249,6 @@ __device__ __forceinline__ void tile_of(int id, int total, int mt, int nt,
 // the other in each wave's half of the tile (the gated layer's two weights).
 template <typename T, int BM, int BN, bool AROWS, bool BROWS, bool SPLITB>
 struct Product {
-
   static constexpr int WM = BM / 2, WN = BN / 2;
   static constexpr int FM = WM / 16, FN = WN / 16;
   static constexpr bool AGPR = FM * FN >= 32;
