@@ -618,6 +618,59 @@ def test_neighbours_of_the_operands_are_not_read_or_written():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("k,n,gated,keep", [
+    (32768, 64, False, None), (64, 32768, False, None),
+    (64, 32768, False, "8bit"), (64, 32768, True, None)])
+def test_more_than_2_to_31_values(k, n, gated, keep):
+    """Small whole numbers: every sum is one below 2**24, exact in float32 in
+    any order, and is rounded once.  In 8 bits, pre-activations of 64 at most
+    keep their sign: one that is not 0 is 2**-6 of its group's largest at
+    least."""
+    m, part = 70016, 8752
+    gen = torch.Generator("cuda").manual_seed(7)
+
+    def whole(*shape):
+        t = torch.empty(*shape, device="cuda", dtype=BF16)
+        for a in range(0, shape[0], part):  # no larger temporary
+            t[a:a + part] = torch.randint(-1, 2, t[a:a + part].shape,
+                                          generator=gen, device="cuda")
+        return t
+
+    x, w, dy = whole(m, k), whole(n * (1 + gated), k), whole(m, n)
+    b = torch.zeros(w.shape[0], device="cuda", dtype=BF16)
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    if gated:
+        y = gated_linear(x, w, b, activation="relu", checkpoint=keep)
+    else:
+        y = linear_act(x, w, b, activation="relu", checkpoint=keep)
+    dx, dw, db = torch.autograd.grad(y, leaves, dy)
+    want_w = torch.zeros(w.shape, device="cuda")
+    want_b = torch.zeros(b.shape, device="cuda")
+    with torch.no_grad():
+        wide = w.float()
+        for a in range(0, m, part):
+            rows = slice(a, a + part)
+            p, d = x[rows].float() @ wide.t(), dy[rows].float()
+            if gated:
+                g, u = p[:, :n], p[:, n:]
+                assert torch.equal(y[rows], (g.clamp(min=0) * u).to(BF16))
+                g = torch.cat([d * u * (g > 0), d * g.clamp(min=0)], 1)
+            else:
+                assert torch.equal(y[rows], p.clamp(min=0).to(BF16))
+                g = d * (p > 0)
+            assert torch.equal(dx[rows], (g @ wide).to(BF16))
+            want_w += g.t() @ x[rows].float()
+            want_b += g.sum(0)
+        assert torch.equal(dw, want_w.to(BF16))
+        assert torch.equal(db, want_b.to(BF16))
+    if x.numel() > 2 ** 31:
+        del y, dx, dw
+        back = unpack_activation(pack_activation(x))
+        for a in range(0, m, part):
+            assert torch.equal(back[a:a + part], x[a:a + part])
+
+
+@pytest.mark.gpu
 def test_on_another_stream():
     x, w, b, r, dy = _make(600, 512, 768, BF16, "cuda", 13, gated=True)
     want = gated_linear(x, w, b)
