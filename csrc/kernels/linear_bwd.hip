@@ -144,7 +144,7 @@ void launch_slope_t(Slope s, hipStream_t st) {
     hipLaunchKernelGGL((slope_kernel<T, kNone, GATED>), grid, block, 0, st, s);
 }
 
-// ---- splits of k -------------------------------------------------------------
+// ---- splits of k ------------------------------------------------------------
 
 // One product's sums of its splits, in their order; blocks from `first` on
 // take the other's.

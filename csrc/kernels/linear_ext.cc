@@ -383,7 +383,7 @@ at::Tensor act8_unpack(at::Tensor codes, at::Tensor scales,
   return x;
 }
 
-// ---- the layers, with autograd -------------------------------------------------
+// ---- the layers, with autograd ----------------------------------------------
 
 namespace {
 

@@ -21,7 +21,8 @@ __device__ __forceinline__ void finish(const P& prod, const Forward& f,
   constexpr int COLS = GATED ? P::WN / 2 : P::WN;
   // The whole residual before the first store, which the compiler has to take
   // for one to the same place: one wait instead of one a row.  Its registers
-  // are the fragments'.
+  // are the fragments'.  Before the products, with their first loads, it costs
+  // as much: 8192 x 768 -> 768 takes 18.0 us so and 16.9 here.
   constexpr int PAIRS = COLS / 32;
   Vec8<T> r[GATED ? 1 : PAIRS][P::FM] = {};
   if constexpr (!GATED) {

@@ -10,7 +10,7 @@ namespace {
 using tile::f32x4;
 using tile::i16x8;
 
-// ---- few rows ------------------------------------------------------------------
+// ---- few rows ---------------------------------------------------------------
 //
 // A block owns 16 rows of the weights (of each projection) and all of x's, up
 // to 32; its eight waves take the k's in turns of 64 and add their sums up
@@ -127,7 +127,7 @@ void rows_by_count(const Forward& f, hipStream_t st) {
   else launch_rows<T, 2, GATED>(f, st);
 }
 
-// ---- splits of k -------------------------------------------------------------
+// ---- splits of k ------------------------------------------------------------
 
 // A thread takes eight columns of a row (and the same of the up half) of all
 // splits, in their order; four threads hold a group of 32 columns.

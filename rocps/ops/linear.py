@@ -4,8 +4,9 @@ The product runs on the matrix cores with fp32 sums; bias, activation and
 residual are applied to the sums before they are rounded once to the type of
 ``x``.  Any number of rows and features, bfloat16 or float16
 (csrc/kernels/linear_fwd.h, linear_rows.hip, linear_bwd.hip on the product of
-tile_gemm.h); on the CPU the same in plain
-PyTorch, in float32 (float64 for float64 inputs).
+tile_gemm.h); on the CPU the same in plain PyTorch, in float32 (float64 for
+float64 inputs).  On the GPU a row has less than 2**22 values and x less than
+2**30 rows; more are refused.
 
 The backward pass keeps ``x`` and, where there is an activation, the
 pre-activations ``p = x W^T + b`` in the type of ``x``, and computes
@@ -18,6 +19,10 @@ bits: g is a product of both, and their rounding to 16 would add as much error
 as that of g itself.)  With ``checkpoint="8bit"`` it keeps x and p in 8 bits
 (rocps/ops/act8.py), half the memory or less: dW and g are then those of the
 kept values; y is the same.
+
+A training step can be captured into a graph.  As for every layer, torch ties
+a leaf's gradient to the stream of the autograd graph that is alive: drop the
+outputs of eager steps on the same weights before the capture.
 """
 
 from __future__ import annotations
