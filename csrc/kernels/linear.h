@@ -40,12 +40,12 @@ struct Forward {
   unsigned char* codes;
   unsigned char* scales;
   long ldp;
+  bool by_rows;  // few rows, on a kernel of their own
   TileChoice choice;
   float* part;  // [splits][m][n or 2n], with splits > 1
 };
-// Few rows take a kernel of their own, which has no splits.
-bool forward_by_rows(const Forward& f);
-TileChoice forward_choice(const Forward& f);
+// Sets by_rows, or choice with splits >= 1.
+void choose_forward(Forward& f);
 void launch_linear_forward(const Forward& f, hipStream_t st);
 void forward_tiles_bf16(const Forward& f, hipStream_t st);
 void forward_tiles_fp16(const Forward& f, hipStream_t st);

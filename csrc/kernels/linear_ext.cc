@@ -165,13 +165,11 @@ static std::tuple<at::Tensor, MaybeTensor, MaybeTensor> linear_forward(
   f.x = xr.p, f.ldx = xr.ld;
   f.w = wr.p, f.ldw = wr.ld;
   at::Tensor part;
-  if (!ff::forward_by_rows(f)) {
-    f.choice = ff::forward_choice(f);
-    if (f.choice.splits > 1) {
-      part = at::empty({f.choice.splits, m, w.size(0)},
-                       x.options().dtype(at::kFloat));
-      f.part = part.data_ptr<float>();
-    }
+  ff::choose_forward(f);
+  if (!f.by_rows && f.choice.splits > 1) {
+    part = at::empty({f.choice.splits, m, w.size(0)},
+                     x.options().dtype(at::kFloat));
+    f.part = part.data_ptr<float>();
   }
   ff::launch_linear_forward(f, st);
   check_launch(op);

@@ -30,6 +30,7 @@ enum Tile { k256x256, k256x128, k128x192, k128x128, k64x128, k64x64, kTiles };
 struct TileChoice {
   Tile tile;
   int splits;
+  double us;
 };
 
 struct TileCost {
@@ -57,7 +58,7 @@ inline long tile_count(const TileCost& t, long m, long n) {
 // those in 8 bits.
 inline TileChoice choose_tile(long m, long n, long k, bool halves, int keep) {
   const long steps = (k + 63) / 64;
-  TileChoice best{k128x128, 1};
+  TileChoice best{k128x128, 1, 0};
   double least = -1;
   for (int i = 0; i < kTiles; i++) {
     const TileCost& t = tile_cost(i);
@@ -77,13 +78,36 @@ inline TileChoice choose_tile(long m, long n, long k, bool halves, int keep) {
       if (s > 1) us += 4 + s * 2e-6 * m * n;
       if (least < 0 || us < least) {
         least = us;
-        best = {(Tile)i, s};
+        best = {(Tile)i, s, us};
       }
       if (tiles * s >= 4 * kCUs) break;
     }
   }
   return best;
 }
+
+// Up to 64 rows have a kernel that goes by 16 columns (linear_rows.hip).  What
+// it takes, in us past the launch: a turn of its own and one of the rows for
+// every k, times the blocks that a CU gets; blocks that share a CU wait for
+// each other's loads.  Against the tiles, of which a few rows fill little and
+// which start more slowly:
+//                           16 rows        32            48
+//   4096 -> 4096            7.6   13.7     8.0   14.6    8.9   15.4 us
+//   8192 -> 2048            9.2   16.5     9.9   16.8    12.2  17.6
+//   4096 -> 16384           26.6  37.2     33.7  37.8    40.8  38.8
+//   1024 -> 32768           16.5  15.4     20.9  15.6    26.6  16.0
+//   gated, 16384 -> 1024    31.3  23.8     38.7  24.6    45.1  25.4
+// Over 24 shapes of both layers and 1 to 48 rows the choice is 1% slower than
+// the better one.
+inline double rows_cost(long m, long n, long k, bool gated) {
+  const int h = gated ? 2 : 1;
+  const long runs = (m + 15) / 16;
+  const double blocks = (double)n / 16 / kCUs;
+  return blocks <= 1 ? 1e-3 * k * h * (0.6 + 0.25 * runs)
+                     : 1e-3 * k * blocks * (1.3 * h + 0.5 * runs);
+}
+
+inline double tiles_for_few(double us) { return 1.2 * us + 2; }
 
 // Two products of one launch, in tiles of one size, the longer ones first: a
 // CU that is done with its share of one goes on with the other, so what

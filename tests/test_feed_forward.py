@@ -581,6 +581,19 @@ def test_larger_sizes(m, k, n, gated):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m,k,n", [
+    (1, 2048, 40), (9, 1030, 33), (16, 8200, 40), (17, 64, 80),
+    (31, 513, 16), (32, 4104, 72), (33, 200, 4097), (48, 1000, 100),
+    (49, 520, 1000), (63, 40, 5000), (64, 3000, 30), (64, 1536, 9000)])
+def test_few_rows(m, k, n):
+    """Each count of 16 rows, k's that end inside a turn or give a wave none,
+    and columns that end inside a block."""
+    for t, gated in ((BF16, False), (FP16, True)):
+        _check(*_make(m, k, n, t, "cuda", n, gated=gated, res=not gated),
+               "gelu", gated)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("gated", [False, True])
 def test_the_same_inputs_give_the_same_bits(gated):
     x, w, b, r, dy = _make(513, 777, 650, BF16, "cuda", 11, gated=gated)
