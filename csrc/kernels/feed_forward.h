@@ -159,24 +159,34 @@ __device__ __forceinline__ float from_24(unsigned hi, unsigned lo) {
 }
 
 using u16x8 = __attribute__((ext_vector_type(8))) unsigned short;
+using u32x2 = __attribute__((ext_vector_type(2))) unsigned;
 
 // ---- 16-bit vectors --------------------------------------------------------
 
 template <typename T> using Vec8 = __attribute__((ext_vector_type(8))) T;
 
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, float* v) {
-  const Vec8<T> u = *(const Vec8<T>*)p;
+template <typename V>
+__device__ __forceinline__ void widen(V u, float* v) {
 #pragma unroll
   for (int k = 0; k < 8; k++) v[k] = (float)u[k];
 }
 
 template <typename T>
-__device__ __forceinline__ void store8(T* p, const float* v) {
+__device__ __forceinline__ void load8(const T* p, float* v) {
+  widen(*(const Vec8<T>*)p, v);
+}
+
+template <typename T>
+__device__ __forceinline__ Vec8<T> to8(const float* v) {
   Vec8<T> u;
 #pragma unroll
   for (int k = 0; k < 8; k++) u[k] = (T)v[k];
-  *(Vec8<T>*)p = u;
+  return u;
+}
+
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float* v) {
+  *(Vec8<T>*)p = to8<T>(v);
 }
 
 // n valid values from an address of any alignment, zeros behind them.  Eight
@@ -197,16 +207,11 @@ __device__ __forceinline__ Vec8<T> some8(const T* p, long n) {
 
 template <typename T>
 __device__ __forceinline__ void load_some(const T* p, long n, float* v) {
-  const Vec8<T> u = some8(p, n);
-#pragma unroll
-  for (int k = 0; k < 8; k++) v[k] = (float)u[k];
+  widen(some8(p, n), v);
 }
 
 template <typename T>
-__device__ __forceinline__ void store_some(T* p, long n, const float* v) {
-  Vec8<T> u;
-#pragma unroll
-  for (int k = 0; k < 8; k++) u[k] = (T)v[k];
+__device__ __forceinline__ void put_some(T* p, long n, Vec8<T> u) {
   if (n >= 8) {
     *(Any8<T>*)p = u;
   } else {
@@ -216,18 +221,21 @@ __device__ __forceinline__ void store_some(T* p, long n, const float* v) {
   }
 }
 
-__device__ __forceinline__ void store24(unsigned short* hi, unsigned char* lo,
-                                        const float* v) {
-  u16x8 h;
+template <typename T>
+__device__ __forceinline__ void store_some(T* p, long n, const float* v) {
+  put_some(p, n, to8<T>(v));
+}
+
+// the 16 upper bits of each, and the next 8 of all
+__device__ __forceinline__ uint2 split24(const float* v, u16x8& hi) {
   unsigned l[2] = {0, 0};
 #pragma unroll
   for (int k = 0; k < 8; k++) {
     const unsigned b = to_24(v[k]);
-    h[k] = (unsigned short)(b >> 8);
+    hi[k] = (unsigned short)(b >> 8);
     l[k >> 2] |= (b & 255u) << (k & 3) * 8;
   }
-  *(u16x8*)hi = h;
-  *(uint2*)lo = make_uint2(l[0], l[1]);
+  return make_uint2(l[0], l[1]);
 }
 
 __device__ __forceinline__ void load24(const unsigned short* hi,

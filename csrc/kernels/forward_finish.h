@@ -12,40 +12,42 @@ enum Keep { kNothing = 0, kPre = 1, k8 = 2 };
 
 // columns n.. of the bias, zeros behind the last one
 template <typename T>
-__device__ __forceinline__ void bias8(const Forward& f, long n, long half,
-                                      float* v) {
-  const T* b = (const T*)f.bias;
-  if (b == nullptr || n >= f.n) {
+__device__ __forceinline__ Vec8<T> bias8(const Forward& f, long n, long half) {
+  if (f.bias == nullptr) return Vec8<T>{};
+  return some8((const T*)f.bias + half + n, f.n - n);
+}
+
+// Codes and exponent of eight pre-activations, columns n..; the lanes X, Y and
+// X + Y away hold the rest of a group of 32 columns.
+template <int X, int Y>
+__device__ __forceinline__ uint2 codes8(const Forward& f, long n,
+                                        const float* v, int& e) {
+  float w[8];
+  const bool whole = n + 8 <= f.n;
 #pragma unroll
-    for (int k = 0; k < 8; k++) v[k] = 0.f;
-  } else if (f.vec_out) {
-    load8(b + half + n, v);
-  } else {
-    load_some(b + half + n, f.n - n, v);
-  }
+  for (int k = 0; k < 8; k++) w[k] = whole || n + k < f.n ? v[k] : 0.f;
+  return encode8<X, Y>(w, e);
 }
 
 // Keeps eight pre-activations of row m, columns n.. of the gated layer's up
-// half or the other.  In 8 bits, the lanes X, Y and X + Y away hold the
-// rest of a group of 32 columns.
+// half or the other.
 template <typename T, int KEEP, bool GATED, int X, int Y>
 __device__ __forceinline__ void keep_pre(const Forward& f, long m, long n,
                                          bool up, bool live, const float* v) {
   const long at = m * f.ldp + (up ? f.ldp / 2 : 0) + n;
   if constexpr (KEEP == kPre) {
     if (live && n < f.n) {
-      if constexpr (GATED)
-        store24((unsigned short*)f.pre + at, f.low + at, v);
-      else
-        store8((T*)f.pre + at, v);
+      if constexpr (GATED) {
+        u16x8 hi;
+        *(uint2*)(f.low + at) = split24(v, hi);
+        *(u16x8*)((unsigned short*)f.pre + at) = hi;
+      } else {
+        *(Vec8<T>*)((T*)f.pre + at) = to8<T>(v);
+      }
     }
   } else if constexpr (KEEP == k8) {
-    float w[8];
-    const bool whole = n + 8 <= f.n;
-#pragma unroll
-    for (int k = 0; k < 8; k++) w[k] = whole || n + k < f.n ? v[k] : 0.f;
     int e;
-    const uint2 codes = encode8<X, Y>(w, e);
+    const uint2 codes = codes8<X, Y>(f, n, v, e);
     if (live && (n & ~31L) < f.n) {
       *(uint2*)(f.codes + at) = codes;
       if ((n & 31) == 0) f.scales[at >> 5] = (unsigned char)(e + 127);
@@ -69,12 +71,8 @@ __device__ __forceinline__ void act8<-1>(float* v, int a) {
 // Eight columns of the residual, zeros where there is none.
 template <typename T>
 __device__ __forceinline__ Vec8<T> residual8(const Forward& f, long m, long n) {
-  Vec8<T> r = {};
-  if (f.res != nullptr && m < f.m && n < f.n) {
-    const T* p = (const T*)f.res + m * f.ldr + n;
-    r = f.vec_out ? *(const Vec8<T>*)p : some8(p, f.n - n);
-  }
-  return r;
+  if (f.res == nullptr || m >= f.m) return Vec8<T>{};
+  return some8((const T*)f.res + m * f.ldr + n, f.n - n);
 }
 
 // v (and the gated layer's u): the products, with the bias; r: the residual.
@@ -92,11 +90,7 @@ __device__ __forceinline__ void finish8(const Forward& f, long m, long n,
     else v[k] += (float)r[k];
   }
   if (!live || n >= f.n) return;
-  T* y = (T*)f.y + m * f.n + n;
-  if (f.vec_out)
-    store8(y, v);
-  else
-    store_some(y, f.n - n, v);
+  store_some((T*)f.y + m * f.n + n, f.n - n, v);
 }
 
 }  // namespace ff

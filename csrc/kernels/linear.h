@@ -19,7 +19,6 @@ constexpr long kMaxPitch = 1L << 22;
 struct Forward {
   int type, act;
   bool gated;
-  bool vec_out;  // n % 8 == 0 and y, bias, residual 16-byte aligned
   long m, n, k;
   const void* x;
   long ldx;
@@ -91,7 +90,6 @@ void launch_slope(const Slope& s, hipStream_t st);
 // aligned with pitches of whole 16 bytes; an operand by k has k in whole 16
 // bytes, its zeros included.
 struct Matmul {
-  bool vec_out;  // n % 8 == 0, out aligned
   long m, n, k;
   const void* a;
   long lda;

@@ -118,7 +118,6 @@ static std::tuple<at::Tensor, MaybeTensor, MaybeTensor> linear_forward(
   f.gated = gated;
   f.m = m, f.n = n, f.k = k;
   f.y = y.data_ptr();
-  f.vec_out = n % 8 == 0;
   at::Tensor b, r;
   if (bias.has_value()) {
     TORCH_CHECK(bias->device() == x.device() &&
@@ -128,7 +127,6 @@ static std::tuple<at::Tensor, MaybeTensor, MaybeTensor> linear_forward(
                 " on ", x.device());
     b = bias->contiguous();
     f.bias = b.data_ptr();
-    f.vec_out = f.vec_out && aligned(f.bias);
   }
   if (res.has_value()) {
     TORCH_CHECK(!gated, op, ": no residual");
@@ -138,7 +136,6 @@ static std::tuple<at::Tensor, MaybeTensor, MaybeTensor> linear_forward(
     r = inner_contiguous(*res);
     f.res = r.data_ptr();
     f.ldr = m > 1 ? r.stride(0) : n;
-    f.vec_out = f.vec_out && aligned(f.res) && f.ldr % 8 == 0;
   }
   MaybeTensor pre, scales;
   if (keep != 0 && act != 0) {
@@ -304,7 +301,6 @@ static std::tuple<MaybeTensor, MaybeTensor, MaybeTensor> linear_backward(
   at::Tensor parts[2];
   for (int i = 0; i < 2; i++) {
     ff::Matmul& p = i == 0 ? q.dx : q.dw;
-    p.vec_out = p.n % 8 == 0;
     p.splits = q.choice.splits[i];
     if (p.splits > 1) {
       parts[i] = at::empty({p.splits, p.m, p.n}, f32);

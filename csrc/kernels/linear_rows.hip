@@ -151,8 +151,8 @@ __global__ __launch_bounds__(64 * kWaves) void rows_kernel(const Forward f) {
   const int m = t >> 1, j = (t & 1) * 8;
   const long n = n0 + j;
   float v[8], u[8];
-  bias8<T>(f, n, 0, v);
-  if constexpr (GATED) bias8<T>(f, n, f.n, u);
+  widen(bias8<T>(f, n, 0), v);
+  if constexpr (GATED) widen(bias8<T>(f, n, f.n), u);
   Vec8<T> r = {};
   if constexpr (!GATED) r = residual8<T>(f, m, n);
 #pragma unroll
@@ -210,8 +210,8 @@ __global__ __launch_bounds__(256) void join_forward_kernel(const Forward f) {
        i += (long)gridDim.x * 256) {
     const long m = i / per, n = (i - m * per) * 8;
     float v[8], u[8];
-    bias8<T>(f, n, 0, v);
-    if constexpr (GATED) bias8<T>(f, n, f.n, u);
+    widen(bias8<T>(f, n, 0), v);
+    if constexpr (GATED) widen(bias8<T>(f, n, f.n), u);
     Vec8<T> r = {};
     if constexpr (!GATED) r = residual8<T>(f, m, n);
     for (int s = 0; s < f.choice.splits; s++) {
@@ -281,7 +281,6 @@ void launch_linear_forward(const Forward& f, hipStream_t st) {
   }
   Matmul q{};
   q.m = f.m, q.n = f.gated ? 2 * f.n : f.n, q.k = f.k;
-  q.vec_out = q.n % 8 == 0;
   q.a = f.x, q.lda = f.ldx;
   q.b = f.w, q.ldb = f.ldw;
   q.part = f.part;

@@ -6,11 +6,56 @@
 #include "feed_forward.h"
 #include "linear.h"
 #include "tile_gemm.h"
+#include "tile_rows.h"
 
 namespace ff {
 
 using tile::Operand;
 using tile::Product;
+
+// A wave's part of a tile, rows from m0 and columns from n0 on, to out[m][n].
+template <typename P, typename O>
+__device__ __forceinline__ void write_tile(const P& prod, char* smem, int wid,
+                                           int lane, O* out, long m0, long n0,
+                                           long m, long n) {
+  using Turn = tile::Turned<P::WN, sizeof(O)>;
+  static_assert(4 * Turn::LDS <= P::LDS, "the waves' rows");
+  constexpr int EACH = 16 / sizeof(O);  // columns a chunk
+  using V = __attribute__((ext_vector_type(EACH))) O;
+  tile::lds_char* const own = (tile::lds_char*)smem + wid * Turn::LDS;
+#pragma unroll
+  for (int i = 0; i < P::FM; i++) {
+#pragma unroll
+    for (int p = 0; p < P::FN / 2; p++) {
+      float v[8];
+      prod.eight(i, p, v);
+      const int c = p * 32 + P::column(lane);
+      V u[8 / EACH];
+#pragma unroll
+      for (int k = 0; k < 8; k++) u[k / EACH][k % EACH] = (O)v[k];
+#pragma unroll
+      for (int k = 0; k < 8 / EACH; k++)
+        Turn::put(own, lane & 15, c + k * EACH, u[k]);
+    }
+#pragma unroll
+    for (int r = 0; r < Turn::READS; r++) {
+      const V u = Turn::template get<V>(own, lane, r);
+      const long row = m0 + i * 16 + Turn::row(lane, r);
+      const long c = n0 + Turn::chunk(lane, r) * EACH;
+      if (row < m && c < n) {
+        O* to = out + row * n + c;
+        if (c + EACH <= n) {
+          typedef V Any __attribute__((aligned(sizeof(O))));
+          *(Any*)to = u;
+        } else {
+#pragma unroll
+          for (int k = 0; k < EACH; k++)
+            if (c + k < n) to[k] = u[k];
+        }
+      }
+    }
+  }
+}
 
 // Block `id` of a product's tiles and splits.
 template <typename T, int BM, int BN, bool AROWS, bool BROWS>
@@ -35,31 +80,13 @@ __device__ __forceinline__ void matmul_block(char* smem, const Matmul& q,
 
   const int lane = threadIdx.x & 63;
   const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const bool whole = q.splits == 1;
-  float* part = q.part + (long)split * q.m * q.n;
-#pragma unroll
-  for (int p = 0; p < P::FN / 2; p++) {
-    const long n = n0 + (wid & 1) * P::WN + p * 32 + P::column(lane);
-#pragma unroll
-    for (int i = 0; i < P::FM; i++) {
-      const long m = m0 + (wid >> 1) * P::WM + i * 16 + (lane & 15);
-      float v[8];
-      prod.eight(i, p, v);
-      if (m >= q.m || n >= q.n) continue;
-      const long at = m * q.n + n;
-      if (whole) {
-        if (q.vec_out)
-          store8((T*)q.out + at, v);
-        else
-          store_some((T*)q.out + at, q.n - n, v);
-      } else if (q.vec_out) {
-        *(tile::f32x4*)(part + at) = tile::f32x4{v[0], v[1], v[2], v[3]};
-        *(tile::f32x4*)(part + at + 4) = tile::f32x4{v[4], v[5], v[6], v[7]};
-      } else {
-        store_some(part + at, q.n - n, v);
-      }
-    }
-  }
+  const long mw = m0 + (wid >> 1) * P::WM, nw = n0 + (wid & 1) * P::WN;
+  tile::barrier();  // the tiles' last reads are done
+  if (q.splits == 1)
+    write_tile<P>(prod, smem, wid, lane, (T*)q.out, mw, nw, q.m, q.n);
+  else
+    write_tile<P>(prod, smem, wid, lane, q.part + (long)split * q.m * q.n, mw,
+                  nw, q.m, q.n);
 }
 
 template <typename T, int BM, int BN, int BLOCKS>
