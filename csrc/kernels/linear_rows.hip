@@ -28,7 +28,8 @@ using tile::i16x8;
 // would all read from a few of the memory's channels at a time (4096 -> 2 x
 // 8192: 29.3 us).
 // (Rows of odd lengths are copied first: read as they lie, 16 bytes at any
-// address, 24 rows of 4095 -> 4095 took 39 us, with the copy of the weights 34.)
+// address, 24 rows of 4095 -> 4095 took 39 us, with the copy of the weights
+// 34.)
 //
 // S turns are in flight.  Two are faster where one row's k is long and no more
 // than one block comes to a CU (16 x 16384 -> 1024: 13.0 us, with one 15.3),
