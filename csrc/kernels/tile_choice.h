@@ -1,26 +1,28 @@
 // Which tile and how many splits of k a product of the tiled kernel takes.
 //
-// Measured on an MI355X, bf16:
-//   tile       blocks   us a step of 64 k's                 us a 256 x 256
-//              a CU     one block   each of all    the same, of the output,
-//                       alone       the CU's, by   by rows   with all CUs
-//                                   k                        at it
-//   256 x 256    1        1.40         1.40         1.45        13
-//   256 x 128    1        0.80         0.80         0.86        15
-//   128 x 192    1        0.61         0.61         0.66        14
-//   128 x 128    2        0.50         0.42         0.45         9
-//    64 x 128    2        0.36         0.27         0.29        12
-//    64 x  64    4        0.34         0.17         0.25         8
+// What a step of 64 k's and a tile's end cost, in us, bf16 on an MI355X:
+//   tile       blocks   a step: one     each of all the CU's,    256 x 256 of
+//              a CU     block alone     by k       by rows       the output
+//   256 x 256    1        1.40          1.23         1.20        12.2
+//   256 x 128    1        0.80          0.69         0.76        13.0
+//   128 x 192    1        0.60          0.54         0.69        13.7
+//   128 x 128    2        0.40          0.39         0.41         8.6
+//    64 x 128    2        0.33          0.27         0.33        12.3
+//    64 x  64    4        0.30          0.17         0.21         9.5
 // and with pre-activations kept, 3 more where one block has the CU and 5 more
-// where they share it; in 8 bits 9 and 8 more.
+// where they share it; in 8 bits 9 and 8 more.  They are within a tenth or so
+// of what single products take, and chosen so that the rules below choose
+// well: over 91 shapes of the forward pass and 90 of the backward pass, of 70
+// to 16384 rows and widths of 200 to 30528, each with every tile and split
+// measured, the choice is 1.7% and 1.3% slower than the best on average.
 // A larger tile does more with what it reads; a smaller one leaves fewer CUs
 // without work at the end, and two blocks on a CU write one's results while
 // they multiply the other's.  The choice is the least time of the fullest CU.
-// For 4096 x 4096 x 8192 (both operands by k) the tiles take 187, 214, 235,
-// 222, 280 and 353 us, for 8192 x 768 x 4096 77, 51, 45, 55, 64 and 71, for
-// 1024 x 1024 x 4096 78, 46, 39, 33, 28 and 26.
-// Splits of k add partial sums in 32 bits, written, read and added up: their
-// bytes at 4 TB/s and 4 us for the launch that joins them.
+// For 4096 x 4096 x 8192 (both operands by k) the tiles take 185, 213, 238,
+// 223, 293 and 369 us, for 8192 x 768 x 4096 73, 51, 46, 52, 68 and 74, for
+// 1024 x 1024 x 4096 71, 45, 38, 34, 30 and 28.
+// Splits of k add partial sums in 32 bits, written, read and added up: 4.5 us
+// for the launch that joins them, and their bytes.
 #pragma once
 
 namespace ff {
@@ -41,13 +43,17 @@ struct TileCost {
 
 inline const TileCost& tile_cost(int t) {
   static const TileCost costs[kTiles] = {
-      {256, 256, 1, 1.40, 1.40, 1.45, 13}, {256, 128, 1, 0.80, 0.80, 0.86, 15},
-      {128, 192, 1, 0.61, 0.61, 0.66, 14}, {128, 128, 2, 0.50, 0.42, 0.45, 9},
-      {64, 128, 2, 0.36, 0.27, 0.29, 12},  {64, 64, 4, 0.34, 0.17, 0.25, 8}};
+      {256, 256, 1, 1.40, 1.23, 1.20, 12.2},
+      {256, 128, 1, 0.80, 0.69, 0.76, 13.0},
+      {128, 192, 1, 0.60, 0.54, 0.69, 13.7},
+      {128, 128, 2, 0.40, 0.39, 0.41, 8.6},
+      {64, 128, 2, 0.33, 0.27, 0.33, 12.3},
+      {64, 64, 4, 0.30, 0.17, 0.21, 9.5}};
   return costs[t];
 }
 
 constexpr long kCUs = 256;
+constexpr double kJoin = 4.5, kJoinEach = 1.3e-6;  // us, and for a value's sum
 
 inline long tile_count(const TileCost& t, long m, long n) {
   return ((m + t.bm - 1) / t.bm) * ((n + t.bn - 1) / t.bn);
@@ -75,7 +81,7 @@ inline TileChoice choose_tile(long m, long n, long k, bool halves, int keep) {
       if (rest != 0) last = rest * t.each > t.alone ? rest * t.each : t.alone;
       double us = ((steps + s - 1) / s) * ((each - rest) * t.each + last);
       us += each * out;
-      if (s > 1) us += 4 + s * 2e-6 * m * n;
+      if (s > 1) us += kJoin + s * kJoinEach * m * n;
       if (least < 0 || us < least) {
         least = us;
         best = {(Tile)i, s, us};
@@ -168,12 +174,12 @@ inline PairChoice choose_pair(const long m[2], const long n[2],
         const long total = tiles[0] * s0 + tiles[1] * s1;
         long share = (total + kCUs - 1) / kCUs;
         share = share < t.per_cu ? share : t.per_cu;
-        const double with = t.rows * (1 + 0.6 * (share - 1));
+        const double with = t.rows * (1 + 0.5 * (share - 1));
         const double lone = most * (with > t.alone ? with : t.alone) + out;
         double us = end > lone ? end : lone;
-        if (s0 > 1 || s1 > 1) us += 4;
-        if (s0 > 1) us += s0 * 2e-6 * m[0] * n[0];
-        if (s1 > 1) us += s1 * 2e-6 * m[1] * n[1];
+        if (s0 > 1 || s1 > 1) us += kJoin;
+        if (s0 > 1) us += s0 * kJoinEach * m[0] * n[0];
+        if (s1 > 1) us += s1 * kJoinEach * m[1] * n[1];
         if (least < 0 || us < least) {
           least = us;
           best = {(Tile)i, {s0, s1}, swap};
