@@ -120,9 +120,15 @@ void launch_backward(const Backward& b, hipStream_t st);
 void backward_tiles_bf16(const Backward& b, hipStream_t st);
 void backward_tiles_fp16(const Backward& b, hipStream_t st);
 
-// rows of `n` 16-bit values to rows of `ldo` >= n, zeros behind
-void launch_repack(const void* x, long ldx, long m, long n, void* out,
-                   long ldo, hipStream_t st);
+// Rows of `n` 16-bit values to rows of `ldo` >= n, zeros behind; none with
+// m = 0.  Both in one launch.
+struct Repack {
+  const void* x;
+  long ldx, m, n;
+  void* out;
+  long ldo;
+};
+void launch_repack(const Repack& a, const Repack& b, hipStream_t st);
 
 void launch_pack(const Pack& p, hipStream_t st);
 void launch_unpack(const Pack& p, hipStream_t st);  // zeros to ldx behind n

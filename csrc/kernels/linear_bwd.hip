@@ -181,15 +181,17 @@ Join join_of(const Matmul& q) {
           count == 0 ? 0 : rocps_grid_for((count + 7) / 8, 256)};
 }
 
-__global__ __launch_bounds__(256) void repack_kernel(const short* x, long ldx,
-                                                     long m, long n,
-                                                     short* out, long ldo) {
-  const long per = ldo / 8, total = m * per;
-  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total;
+__global__ __launch_bounds__(256) void repack_kernel(const Repack a,
+                                                     const Repack b) {
+  const long first = a.m * (a.ldo / 8), all = first + b.m * (b.ldo / 8);
+  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < all;
        i += (long)gridDim.x * 256) {
-    const long r = i / per, c = (i - r * per) * 8;
-    const Vec8<short> v = some8(x + r * ldx + c, n - c);
-    *(Vec8<short>*)(out + r * ldo + c) = v;
+    const bool one = i < first;
+    const Repack p = one ? a : b;
+    const long j = one ? i : i - first, per = p.ldo / 8;
+    const long r = j / per, c = (j - r * per) * 8;
+    *(Vec8<short>*)((short*)p.out + r * p.ldo + c) =
+        some8((const short*)p.x + r * p.ldx + c, p.n - c);
   }
 }
 
@@ -228,11 +230,11 @@ void launch_backward(const Backward& q, hipStream_t st) {
     hipLaunchKernelGGL((join_kernel<_Float16>), grid, block, 0, st, a, b);
 }
 
-void launch_repack(const void* x, long ldx, long m, long n, void* out,
-                   long ldo, hipStream_t st) {
-  hipLaunchKernelGGL(repack_kernel, dim3(rocps_grid_for(m * (ldo / 8), 256)),
-                     dim3(256), 0, st, (const short*)x, ldx, m, n,
-                     (short*)out, ldo);
+void launch_repack(const Repack& a, const Repack& b, hipStream_t st) {
+  const long all = a.m * (a.ldo / 8) + b.m * (b.ldo / 8);
+  if (all == 0) return;
+  hipLaunchKernelGGL(repack_kernel, dim3(rocps_grid_for(all, 256)), dim3(256),
+                     0, st, a, b);
 }
 
 }  // namespace ff

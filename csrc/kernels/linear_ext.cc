@@ -49,10 +49,13 @@ struct Rows {
   at::Tensor keep;
   const void* p;
   long ld;
+  at::Tensor from;  // what `keep` is to be a copy of
 };
 
-// `n` of its columns: a copy that is one already has more.
-Rows whole_rows(const at::Tensor& t, long n, hipStream_t st, const char* op) {
+// `n` of its columns: a copy that is one already has more.  What is to be
+// copied goes to `todo`.
+Rows whole_rows(const at::Tensor& t, long n, ff::Repack& todo,
+                const char* op) {
   const long m = t.size(0);
   if (t.size(1) != n) return {t, t.data_ptr(), t.stride(0)};
   TORCH_CHECK(n < ff::kMaxPitch, op, ": a row of ", n, " is too long");
@@ -64,9 +67,8 @@ Rows whole_rows(const at::Tensor& t, long n, hipStream_t st, const char* op) {
     return {u, u.data_ptr(), ld};
   const long ldo = up_to(n, 8);
   auto out = at::empty({m, ldo}, t.options());
-  ff::launch_repack(u.data_ptr(), m > 1 ? u.stride(0) : n, m, n,
-                    out.data_ptr(), ldo, st);
-  return {out, out.data_ptr(), ldo};
+  todo = {u.data_ptr(), m > 1 ? u.stride(0) : n, m, n, out.data_ptr(), ldo};
+  return {out, out.data_ptr(), ldo, u};
 }
 
 // rows of any alignment, their values side by side
@@ -156,7 +158,10 @@ static std::tuple<at::Tensor, MaybeTensor, MaybeTensor> linear_forward(
   }
   if (m == 0) return {y, pre, scales};
   TORCH_CHECK(m < (1L << 30), op, ": ", m, " rows are too many");
-  const Rows xr = whole_rows(x, k, st, op), wr = whole_rows(w, k, st, op);
+  ff::Repack copies[2] = {};
+  const Rows xr = whole_rows(x, k, copies[0], op);
+  const Rows wr = whole_rows(w, k, copies[1], op);
+  ff::launch_repack(copies[0], copies[1], st);
   if (x_used != nullptr) *x_used = xr.keep;
   if (w_used != nullptr) *w_used = wr.keep;
   f.x = xr.p, f.ldx = xr.ld;
@@ -244,6 +249,7 @@ static std::tuple<MaybeTensor, MaybeTensor, MaybeTensor> linear_backward(
     s.sums = sums.data_ptr<float>();
   }
   Rows wr, xr;
+  ff::Repack copies[2] = {};
   if (need_w) {
     TORCH_CHECK(x.has_value(), op, ": no input");
     if (x_scales.has_value()) {
@@ -263,9 +269,17 @@ static std::tuple<MaybeTensor, MaybeTensor, MaybeTensor> linear_backward(
     } else {
       check_2d(*x, dy, op, "x");
       TORCH_CHECK(fits(*x, m, k), op, ": no input of this gradient's shape");
-      xr = whole_rows(*x, k, st, op);
+      xr = whole_rows(*x, k, copies[0], op);
     }
   }
+  if (need_x) {
+    TORCH_CHECK(w.has_value(), op, ": no weight");
+    check_2d(*w, dy, op, "weight");
+    TORCH_CHECK(fits(*w, outs, k), op,
+                ": no weight of this gradient's shape");
+    wr = whole_rows(*w, k, copies[1], op);
+  }
+  ff::launch_repack(copies[0], copies[1], st);
   ff::launch_slope(s, st);
 
   // ---- the products, and the bias gradient's last sums
@@ -278,11 +292,6 @@ static std::tuple<MaybeTensor, MaybeTensor, MaybeTensor> linear_backward(
     q.dbias = db->data_ptr();
   }
   if (need_x) {
-    TORCH_CHECK(w.has_value(), op, ": no weight");
-    check_2d(*w, dy, op, "weight");
-    TORCH_CHECK(fits(*w, outs, k), op,
-                ": no weight of this gradient's shape");
-    wr = whole_rows(*w, k, st, op);
     q.dx.m = m, q.dx.n = k, q.dx.k = outs;
     q.dx.a = gp, q.dx.lda = ldg;
     q.dx.b = wr.p, q.dx.ldb = wr.ld;
