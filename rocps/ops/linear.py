@@ -18,7 +18,8 @@ db from the unrounded g.  (The gated layer keeps its two projections in 24
 bits: g is a product of both, and their rounding to 16 would add as much error
 as that of g itself.)  With ``checkpoint="8bit"`` it keeps x and p in 8 bits
 (rocps/ops/act8.py), half the memory or less: dW and g are then those of the
-kept values; y is the same.
+kept values.  y is the same but for the order of its sums, which goes by sizes
+and by what is kept.
 
 A training step can be captured into a graph.  As for every layer, torch ties
 a leaf's gradient to the stream of the autograd graph that is alive: drop the

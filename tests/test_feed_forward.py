@@ -697,6 +697,59 @@ def test_on_another_stream():
 
 
 @pytest.mark.gpu
+def test_two_streams_at_once():
+    """Calls that overlap share no workspace: splits of k, copies of odd rows,
+    few rows and training, each on its own stream, over and over."""
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    made = [_make(m, k, n, BF16, "cuda", m, gated=g)
+            for m, k, n, g in ((600, 2049, 300, False), (40, 1111, 500, True),
+                               (1500, 512, 264, True), (7, 4096, 96, False))]
+
+    def step(i):
+        x, w, b, _, dy = made[i]
+        ls = [v.detach().requires_grad_() for v in (x, w, b)]
+        y = (gated_linear(*ls) if i in (1, 2)
+             else linear_act(*ls, activation="gelu"))
+        return [y.detach(), *torch.autograd.grad(y, ls, dy)]
+
+    want = [step(i) for i in range(len(made))]
+    torch.cuda.synchronize()
+    got = []
+    for turn in range(6):
+        for i in range(len(made)):
+            s = streams[(turn + i) % 2]
+            with torch.cuda.stream(s):
+                got.append((i, step(i)))
+    torch.cuda.synchronize()
+    for i, out in got:
+        for p, q in zip(out, want[i]):
+            assert torch.equal(p, q)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [1, 24, 64])
+def test_captured_few_rows(m):
+    x, w, b, _, _ = _make(m, 1500, 700, BF16, "cuda", m, gated=True)
+    v = torch.randn(1500, 700, device="cuda").to(BF16) / 26
+
+    def block(x):
+        with torch.no_grad():
+            return linear_act(gated_linear(x, w, b), v, None, x)
+
+    block(x)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = block(x)
+    for _ in range(4):
+        new = torch.randn(m, 1500, device="cuda").to(BF16)
+        x.copy_(new)
+        g.replay()
+        assert torch.equal(out, block(new))
+        torch.cuda.synchronize()
+
+
+@pytest.mark.gpu
 def test_captured_training_step():
     """A feed-forward block's step in a graph, replayed on new inputs, against
     the eager step; two graphs share nothing."""
