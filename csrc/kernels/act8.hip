@@ -46,7 +46,9 @@ void launch_pack(const Pack& p, hipStream_t st) {
 }
 
 void launch_unpack(const Pack& p, hipStream_t st) {
-  const dim3 grid(rocps_grid_for(p.m * ((p.ldx + 7) / 8), 256, 4096));
+  const int each = p.type == 2 ? 4 : 8;
+  const dim3 grid(
+      rocps_grid_for(p.m * ((p.ldx + each - 1) / each), 256, 4096));
   const dim3 block(256);
   if (p.type == 0)
     hipLaunchKernelGGL((unpack_kernel<__bf16>), grid, block, 0, st, p);

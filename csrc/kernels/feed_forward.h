@@ -127,19 +127,21 @@ __device__ __forceinline__ uint2 encode8(const float* v, int& e) {
   return make_uint2((unsigned)lo, (unsigned)hi);
 }
 
-__device__ __forceinline__ void decode8(uint2 c, unsigned char scale,
+__device__ __forceinline__ void decode4(unsigned c, unsigned char scale,
                                         float* v) {
   const float s = two_to((int)scale - 127);
   using f32x2 = __attribute__((ext_vector_type(2))) float;
   f32x2 p;
-  p = __builtin_amdgcn_cvt_pk_f32_fp8(c.x, false);
+  p = __builtin_amdgcn_cvt_pk_f32_fp8(c, false);
   v[0] = p[0] * s, v[1] = p[1] * s;
-  p = __builtin_amdgcn_cvt_pk_f32_fp8(c.x, true);
+  p = __builtin_amdgcn_cvt_pk_f32_fp8(c, true);
   v[2] = p[0] * s, v[3] = p[1] * s;
-  p = __builtin_amdgcn_cvt_pk_f32_fp8(c.y, false);
-  v[4] = p[0] * s, v[5] = p[1] * s;
-  p = __builtin_amdgcn_cvt_pk_f32_fp8(c.y, true);
-  v[6] = p[0] * s, v[7] = p[1] * s;
+}
+
+__device__ __forceinline__ void decode8(uint2 c, unsigned char scale,
+                                        float* v) {
+  decode4(c.x, scale, v);
+  decode4(c.y, scale, v + 4);
 }
 
 // ---- pre-activations in 24 bits ---------------------------------------------
