@@ -33,8 +33,9 @@ __device__ __forceinline__ float act(float v) {
   return v;
 }
 
-// d act / dv.  Past |v| = 12 the tanh form's slope is 0 or 1 to fp32; the
-// comparisons hold v there, so that v^3 stays finite, and pass NaN on.
+// d act / dv.  Past |v| = 12 the tanh form's slope is 0 or 1 to fp32, and past
+// 100 silu's; the comparisons hold v there, so that v^3 and, where v was kept
+// in fp16 and is infinite there, v itself stay finite, and pass NaN on.
 template <int a>
 __device__ __forceinline__ float slope(float v) {
   if (a == kGelu) {
@@ -45,6 +46,8 @@ __device__ __forceinline__ float slope(float v) {
     return z + (1.f - z) * z * v * __builtin_fmaf(w, kGelu6A, kGelu2C);
   }
   if (a == kSilu) {
+    v = v > 100.f ? 100.f : v;
+    v = v < -100.f ? -100.f : v;
     const float z = sigmoid2(v * kLog2E);
     return z * (1.f + v * (1.f - z));
   }

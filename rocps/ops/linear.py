@@ -61,7 +61,9 @@ def slope_cpu(v: torch.Tensor, act: int) -> torch.Tensor:
         t = torch.tanh(_C * (v + _A * v ** 3))
         return (0.5 * (1 + t)
                 + 0.5 * v * (1 - t * t) * _C * (1 + 3 * _A * v ** 2))
-    if act == 3:
+    if act == 3:  # 0 or 1 at the infinities that a 16-bit type may hold
+        most = torch.finfo(v.dtype).max
+        v = v.clamp(-most, most)
         z = torch.sigmoid(v)
         return z * (1 + v * (1 - z))
     return torch.ones_like(v)

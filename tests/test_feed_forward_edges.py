@@ -1,0 +1,52 @@
+"""The feed-forward operators at the ends of their types and of what they
+take: values past the kept type's range, derivatives that they do not have,
+lengths at their limits, and every kernel that a choice can lead to."""
+
+import pytest
+import torch
+
+from rocps.ops.linear import linear_act
+
+BF16, FP16 = torch.bfloat16, torch.float16
+
+
+def _devices():
+    return ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+
+
+@pytest.mark.parametrize("device", _devices())
+@pytest.mark.parametrize("keep", [None, "8bit"])
+@pytest.mark.parametrize("act", ["relu", "gelu", "silu"])
+def test_slopes_past_the_kept_types_range(act, keep, device):
+    """Pre-activations of +-80000 are finite in float32 and infinite in
+    float16, the type that they are kept in.  There the slope is 1 or 0, and
+    the gradients are sums of a few whole numbers: exact in any order."""
+    k, n = 8, 16
+    s = torch.tensor([1.0, -1.0, 1.0, -1.0])
+    x = (100 * s)[:, None].expand(4, k).to(FP16).to(device).contiguous()
+    w = torch.full((n, k), 100.0, dtype=FP16, device=device)
+    b = torch.zeros(n, dtype=FP16, device=device)
+    ls = [v.requires_grad_() for v in (x, w, b)]
+    y = linear_act(*ls, activation=act, checkpoint=keep)
+    assert torch.equal(y[1::2], torch.zeros_like(y[1::2]))
+    assert (y[::2] == float("inf")).all()  # past float16
+    dx, dw, db = torch.autograd.grad(y, ls, torch.ones_like(y))
+    assert torch.equal(dx[::2], torch.full_like(dx[::2], n * 100.0))
+    assert torch.equal(dx[1::2], torch.zeros_like(dx[1::2]))
+    # two rows of slope 1
+    if keep is None:
+        assert torch.equal(dw, torch.full_like(dw, 200.0))
+    else:  # 100 * 2**2 lies halfway between 384 and 416 and goes to the even
+        assert torch.equal(dw, torch.full_like(dw, 192.0))
+    assert torch.equal(db, torch.full_like(db, 2.0))
+
+
+@pytest.mark.parametrize("device", _devices())
+def test_slopes_pass_not_a_number_on(device):
+    x = torch.tensor([[float("nan")], [1.0]], dtype=FP16, device=device,
+                     requires_grad=True)
+    w = torch.ones(8, 1, dtype=FP16, device=device)
+    for act in ("gelu", "silu"):
+        y = linear_act(x, w, activation=act)
+        dx, = torch.autograd.grad(y, x, torch.ones_like(y))
+        assert dx[0].isnan().all() and dx[1].isfinite().all(), act
