@@ -8,8 +8,9 @@
 
 namespace ff {
 
-// Pitches of operands of the tiled product stay under this many elements, so
-// that a tile's extent is within a 31-bit buffer descriptor.
+// Pitches of operands of the tiled product, filled to whole 16 bytes, stay
+// under this many elements, so that a tile's extent is within a 31-bit buffer
+// descriptor.
 constexpr long kMaxPitch = 1L << 22;
 
 // y = act(x W^T + bias) + residual; with `gated`, W = [Wg; Wu] of 2n rows and

@@ -58,7 +58,8 @@ Rows whole_rows(const at::Tensor& t, long n, ff::Repack& todo,
                 const char* op) {
   const long m = t.size(0);
   if (t.size(1) != n) return {t, t.data_ptr(), t.stride(0)};
-  TORCH_CHECK(n < ff::kMaxPitch, op, ": a row of ", n, " is too long");
+  TORCH_CHECK(up_to(n, 8) < ff::kMaxPitch, op, ": a row of ", n,
+              " is too long");
   at::Tensor u = n > 1 && t.stride(1) != 1 ? t.contiguous() : t;
   const long ld = m > 1 ? u.stride(0) : up_to(n, 8);
   // ld < n: rows that overlap, as an expanded tensor's

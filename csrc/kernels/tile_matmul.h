@@ -13,6 +13,10 @@ namespace ff {
 using tile::Operand;
 using tile::Product;
 
+// 256 rows of the longest pitch end before the offset that loads nothing.
+static_assert(256 * (kMaxPitch - 8) * 2 + tile::LEAD < tile::PAST,
+              "a tile's extent");
+
 // A wave's part of a tile, rows from m0 and columns from n0 on, to out[m][n].
 template <typename P, typename O>
 __device__ __forceinline__ void write_tile(const P& prod, char* smem, int wid,

@@ -50,3 +50,43 @@ def test_slopes_pass_not_a_number_on(device):
         y = linear_act(x, w, activation=act)
         dx, = torch.autograd.grad(y, x, torch.ones_like(y))
         assert dx[0].isnan().all() and dx[1].isfinite().all(), act
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("k", [2 ** 22 - 7, 2 ** 22 - 1, 2 ** 22])
+def test_rows_that_are_too_long_are_refused(k):
+    """Filled to whole 16 bytes, these have 2**22 values; a tile's 256 rows of
+    them would pass the extent that its loads are checked against."""
+    x = torch.zeros(1, k, dtype=BF16, device="cuda")
+    for m in (1, 65):
+        with pytest.raises(RuntimeError, match="too long"):
+            linear_act(x.expand(m, k), x)
+    with pytest.raises(RuntimeError, match="too long"):
+        linear_act(x.clone().requires_grad_(), x, checkpoint="8bit")
+
+
+@pytest.mark.gpu
+def test_the_longest_rows():
+    """Values of -1, 0 and 1: every sum is a whole number below 2**24, exact
+    in float32 in any order, and those of the gradients are at most 256."""
+    k, m, part = 2 ** 22 - 8, 256, 2 ** 19
+    gen = torch.Generator("cuda").manual_seed(1)
+
+    def whole(*shape):
+        t = torch.empty(shape, dtype=torch.int8, device="cuda")
+        return t.random_(-1, 2, generator=gen).to(BF16)
+
+    x, w, dy = whole(m, k), whole(m, k), whole(m, m)
+    few = linear_act(x[:3], w)
+    y = linear_act(x.requires_grad_(), w.requires_grad_())
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    want = torch.zeros(m, m, device="cuda")
+    d = dy.float()
+    with torch.no_grad():
+        for a in range(0, k, part):
+            xs, ws = x[:, a:a + part].float(), w[:, a:a + part].float()
+            want += xs @ ws.t()
+            assert torch.equal(dx[:, a:a + part].float(), d @ ws)
+            assert torch.equal(dw[:, a:a + part].float(), d.t() @ xs)
+    assert torch.equal(y.float(), want.to(BF16).float())
+    assert torch.equal(few, y[:3])
