@@ -509,6 +509,12 @@ at::Tensor linear_layer(at::Tensor x, at::Tensor w, MaybeTensor bias,
                       ": residual ", res->sizes(), ", not ",
                       at::IntArrayRef(shape));
   }
+  // without this they would be lost where no input requires a gradient
+  for (const at::Tensor* t : {&x, &w, bias ? &*bias : nullptr,
+                              res ? &*res : nullptr})
+    TORCH_CHECK_NOT_IMPLEMENTED(
+        t == nullptr || !t->_fw_grad(0).defined(), op,
+        ": no forward-mode derivatives");
   const bool flat = x.dim() == 2;
   long m = 1;
   for (int i = 0; i + 1 < x.dim(); i++) m *= x.size(i);

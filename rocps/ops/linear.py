@@ -221,6 +221,7 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor,
     of one type on one device; ``activation`` None, "relu", "gelu" (tanh form)
     or "silu"; ``checkpoint`` None or "8bit" (see the module).  Rows may have
     any stride; whole multiples of 8 features from 16-byte aligned rows are
-    used where they lie, others are copied first.  Differentiable once."""
+    used where they lie, others are copied first.  Differentiable once,
+    backward; inputs with forward-mode tangents are refused."""
     return layer("linear_act", _ACTS, x, weight, bias, residual, activation,
                  checkpoint, False)

@@ -5,6 +5,7 @@ lengths at their limits, and every kernel that a choice can lead to."""
 import pytest
 import torch
 
+from rocps.ops.gated import gated_linear
 from rocps.ops.linear import linear_act
 
 BF16, FP16 = torch.bfloat16, torch.float16
@@ -90,3 +91,30 @@ def test_the_longest_rows():
             assert torch.equal(dw[:, a:a + part].float(), d.t() @ xs)
     assert torch.equal(y.float(), want.to(BF16).float())
     assert torch.equal(few, y[:3])
+
+
+@pytest.mark.parametrize("device", _devices())
+@pytest.mark.parametrize("grads", [False, True])
+def test_forward_mode_is_refused(grads, device):
+    """A tangent of any input raises; it is never dropped."""
+    import torch.autograd.forward_ad as forward
+
+    def inputs(gated):
+        shapes = [(4, 8), (12, 8), (12,), (4, 12)][:3 if gated else 4]
+        return [torch.ones(s, dtype=BF16, device=device) for s in shapes]
+
+    for gated in (False, True):
+        layer = gated_linear if gated else linear_act
+        for i in range(3 if gated else 4):
+            v = inputs(gated)
+            with forward.dual_level():
+                v[i] = forward.make_dual(v[i], torch.ones_like(v[i]))
+                if grads:
+                    for j, t in enumerate(v):
+                        if j != i:
+                            t.requires_grad_()
+                with pytest.raises(NotImplementedError):
+                    layer(*v)
+                with torch.no_grad(), pytest.raises(NotImplementedError):
+                    layer(*v)
+        layer(*inputs(gated))
