@@ -159,6 +159,8 @@ static std::tuple<at::Tensor, MaybeTensor, MaybeTensor> linear_forward(
   }
   if (m == 0) return {y, pre, scales};
   TORCH_CHECK(m < (1L << 30), op, ": ", m, " rows are too many");
+  TORCH_CHECK(keep == 0 || up_to(w.size(0), 8) < ff::kMaxPitch, op, ": ",
+              w.size(0), " features are too many for a backward pass");
   ff::Repack copies[2] = {};
   const Rows xr = whole_rows(x, k, copies[0], op);
   const Rows wr = whole_rows(w, k, copies[1], op);

@@ -5,8 +5,9 @@ residual are applied to the sums before they are rounded once to the type of
 ``x``.  Any number of rows and features, bfloat16 or float16
 (csrc/kernels/linear_fwd.h, linear_rows.hip, linear_bwd.hip on the product of
 tile_gemm.h); on the CPU the same in plain PyTorch, in float32 (float64 for
-float64 inputs).  On the GPU a row has at most 2**22 - 8 values and x less than
-2**30 rows; more are refused.
+float64 inputs).  On the GPU a row has at most 2**22 - 8 values, x less than
+2**30 rows and, in training, the weight 2**22 - 8 rows at most; more are
+refused.
 
 The backward pass keeps ``x`` and, where there is an activation, the
 pre-activations ``p = x W^T + b`` in the type of ``x``, and computes

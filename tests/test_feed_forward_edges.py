@@ -118,3 +118,39 @@ def test_forward_mode_is_refused(grads, device):
                 with torch.no_grad(), pytest.raises(NotImplementedError):
                     layer(*v)
         layer(*inputs(gated))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act,gated", [(None, False), ("relu", False),
+                                       ("relu", True)])
+def test_features_that_no_backward_pass_takes(act, gated):
+    """More than 2**22 - 8 rows of the weight: used without gradients, refused
+    before the forward pass with them, and at the limit trained.  Whole
+    numbers below 2**24 are exact in float32."""
+    def run(x, w):
+        if gated:
+            return gated_linear(x, w, activation=act)
+        return linear_act(x, w, activation=act)
+
+    gen = torch.Generator("cuda").manual_seed(2)
+    for outs in (2 ** 22 - 8, 2 ** 22 - 6, 2 ** 22):
+        w = torch.randint(-1, 2, (outs, 1), generator=gen, device="cuda")
+        w = w.to(BF16)
+        x = torch.tensor([[1.0], [-2.0], [0.0]], dtype=BF16, device="cuda")
+        p = x.float() @ w.t().float()
+        a, u = (p.chunk(2, 1) if gated else (p, None))
+        want = a.clamp(min=0) if act else a
+        y = run(x, w)
+        assert torch.equal(y.float(), want * u if gated else want)
+        ls = [x.requires_grad_(), w.requires_grad_()]
+        if outs > 2 ** 22 - 8:
+            with pytest.raises(RuntimeError, match="too many"):
+                run(x, w)
+            assert run(x[:0], w).shape == (0, y.shape[1])
+            continue
+        dx, dw = torch.autograd.grad(run(x, w), ls, torch.ones_like(y))
+        s = (a > 0).float() if act else torch.ones_like(a)
+        g = torch.cat([u * s, want], 1) if gated else s
+        with torch.no_grad():
+            assert torch.equal(dx.float(), (g @ w.float()).to(BF16).float())
+            assert torch.equal(dw.float(), g.t() @ x.float())
