@@ -31,9 +31,11 @@ flags.DEFINE_string("model", "resnet50", "mnist_mlp|resnet50|"
 flags.DEFINE_integer("train_steps", 100, "global steps")
 flags.DEFINE_integer("batch_size", 64, "per-worker batch size")
 flags.DEFINE_integer("seq_len", 128, "sequence length (bert)")
-flags.DEFINE_string("feed_forward", "gelu", "bert: gelu|geglu|swiglu")
+flags.DEFINE_string("feed_forward", "gelu", "bert: gelu|geglu|swiglu (the "
+                                            "last two not in fp32 on a GPU)")
 flags.DEFINE_string("act_checkpoint", "", "bert: 8bit keeps the feed-forward "
-                                          "blocks' activations in 8 bits")
+                                          "blocks' activations in 8 bits (not "
+                                          "in fp32 on a GPU)")
 flags.DEFINE_float("learning_rate", 0.1, "base learning rate")
 flags.DEFINE_float("momentum", 0.9, "momentum (conv nets)")
 flags.DEFINE_string("checkpoint_dir", "", "chief checkpoint dir")
@@ -62,8 +64,26 @@ def make_batch(model_name, batch, seq_len, step, seed, device):
     return x, y.to(device)
 
 
+def bert_args(feed_forward, act_checkpoint, dtype, gpu):
+    """The model's arguments for these flags."""
+    if gpu and dtype != "bf16" and (feed_forward != "gelu" or act_checkpoint):
+        raise ValueError(
+            f"--dtype={dtype}: --feed_forward={feed_forward} "
+            f"--act_checkpoint={act_checkpoint} run in 16 bits on a GPU; "
+            "take --dtype=bf16, or the default feed-forward block")
+    kw = {"feed_forward": feed_forward,
+          "act_checkpoint": act_checkpoint or None}
+    if feed_forward != "gelu":
+        kw["intermediate"] = 2048  # two thirds: as many parameters
+    return kw
+
+
 def main(_):
     from rocps.models import build_model
+    kw = {}
+    if FLAGS.model == "bert_base" and FLAGS.job_name != "ps":
+        kw = bert_args(FLAGS.feed_forward, FLAGS.act_checkpoint, FLAGS.dtype,
+                       torch.cuda.is_available())
     cluster = rocps.train.ClusterSpec({
         "ps": [h for h in FLAGS.ps_hosts.split(",") if h],
         "worker": [h for h in FLAGS.worker_hosts.split(",") if h],
@@ -80,12 +100,6 @@ def main(_):
     is_chief = FLAGS.task_index == 0
     torch.manual_seed(FLAGS.seed)
     torch.backends.cudnn.benchmark = True
-    kw = {}
-    if FLAGS.model == "bert_base":
-        kw = {"feed_forward": FLAGS.feed_forward,
-              "act_checkpoint": FLAGS.act_checkpoint or None}
-        if FLAGS.feed_forward != "gelu":
-            kw["intermediate"] = 2048  # two thirds: as many parameters
     model = build_model(FLAGS.model, **kw)
     if torch.cuda.is_available():
         if FLAGS.dtype == "bf16":

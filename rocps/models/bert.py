@@ -16,6 +16,9 @@ layer to the framework's own operators (rocps.ops.linear, rocps.ops.gated):
   parameter count);
 - ``act_checkpoint="8bit"``: the block's activations are kept in 8 bits for
   the backward pass, which halves the memory that they take.
+
+On the GPU these take bfloat16 or float16 models; others are refused by the
+first forward pass.
 """
 
 from __future__ import annotations

@@ -154,3 +154,37 @@ def test_features_that_no_backward_pass_takes(act, gated):
         with torch.no_grad():
             assert torch.equal(dx.float(), (g @ w.float()).to(BF16).float())
             assert torch.equal(dw.float(), g.t() @ x.float())
+
+
+def test_dist_train_refuses_what_the_gpu_does_not_run():
+    """A gated block or 8-bit checkpoints in fp32 on a GPU: the script says so
+    before it starts a server.  (torch is told that there is a GPU.)"""
+    import os
+    import subprocess
+    import sys
+    root = os.path.join(os.path.dirname(__file__), "..")
+
+    def run(code, *args):
+        return subprocess.run(
+            [sys.executable, "-c", "import runpy, sys, torch\n" + code, *args],
+            cwd=root, capture_output=True, text=True, timeout=120)
+
+    r = run("torch.cuda.is_available = lambda: True\n"
+            "runpy.run_path('examples/dist_train.py', run_name='__main__')",
+            "--model=bert_base", "--dtype=fp32", "--feed_forward=geglu",
+            "--job_name=worker", "--worker_hosts=127.0.0.1:1")
+    assert r.returncode != 0 and "--dtype=bf16" in r.stderr, r.stderr
+    r = run("args = runpy.run_path('examples/dist_train.py')['bert_args']\n"
+            "for gpu in (False, True):\n"
+            "    for dtype in ('bf16', 'fp32'):\n"
+            "        for ff in ('gelu', 'geglu', 'swiglu'):\n"
+            "            for keep in ('', '8bit'):\n"
+            "                try:\n"
+            "                    kw = args(ff, keep, dtype, gpu)\n"
+            "                    wide = kw.get('intermediate', 0)\n"
+            "                    assert kw['act_checkpoint'] == (keep or None)\n"
+            "                    assert wide == (0 if ff == 'gelu' else 2048)\n"
+            "                    print('y', end='')\n"
+            "                except ValueError:\n"
+            "                    print('n', end='')\n")
+    assert r.stdout == 18 * "y" + "y" + 5 * "n", r.stderr
