@@ -208,7 +208,8 @@ __device__ __forceinline__ void barrier() {
 // (one idle one more to each load costs 2% to 8%), M0 is set for four loads
 // and their lanes' offsets are ready.
 __device__ __forceinline__ void set_m0(lds_char* dst) {
-  asm volatile("s_mov_b32 m0, %0" : : "s"((unsigned)(unsigned long)dst));
+  asm volatile("s_mov_b32 m0, %0" : : "s"((unsigned)(unsigned long)dst)
+               : "m0");
 }
 
 template <int AT>
