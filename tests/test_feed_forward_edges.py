@@ -7,6 +7,7 @@ import torch
 
 from rocps.ops.gated import gated_linear
 from rocps.ops.linear import linear_act
+from test_feed_forward import _H, _act, _kept8, _round, _slope
 
 BF16, FP16 = torch.bfloat16, torch.float16
 
@@ -188,3 +189,96 @@ def test_dist_train_refuses_what_the_gpu_does_not_run():
             "                except ValueError:\n"
             "                    print('n', end='')\n")
     assert r.stdout == 18 * "y" + "y" + 5 * "n", r.stderr
+
+
+def _held(v):
+    """What 8 bits give back of v: its finite values by their definition, the
+    others as NaN."""
+    fine = v.isfinite()
+    return torch.where(fine, _kept8(torch.where(fine, v, 0.0))[0],
+                       float("nan"))
+
+
+@pytest.mark.parametrize("device", _devices())
+@pytest.mark.parametrize("m,k,n,gated", [
+    (70, 64, 48, False), (70, 64, 48, True), (300, 72, 136, False),
+    (66, 1334, 40, False), (72, 1160, 33, True)])  # the last two: k split
+def test_infinite_pre_activations_in_8_bits(m, k, n, gated, device):
+    """Products of 2**100 and +-2**100 make two columns of the odd rows
+    infinite; their neighbours in the group of 32 are kept as if they were not
+    there, and only gradients that use them are NaN.  Everything else is a
+    whole number of eighths, exact in float32."""
+    gen = torch.Generator().manual_seed(k)
+    outs = 2 * n if gated else n
+
+    def whole(a, b, *s):
+        return torch.randint(a, b, s, generator=gen).double()
+
+    X, W = whole(-9, 10, m, k), whole(-1, 2, outs, k) / 8
+    D = torch.randn(m, n, generator=gen).to(BF16).double()
+    W[:, 0], X[:, 0] = 0, 0
+    W[5, 0], W[n + 6 if gated else 6, 0] = 2.0 ** 100, -2.0 ** 100
+    X[1::2, 0] = 2.0 ** 100
+    P = X @ W.t()
+    P[P.abs() > 2.0 ** 128] *= float("inf")
+    assert (~P.isfinite()).sum() == 2 * (m // 2)
+    x, w, dy = (v.to(BF16).to(device) for v in (X, W, D))
+    ls = [x.requires_grad_(), w.requires_grad_()]
+    if gated:
+        y = gated_linear(*ls, activation="silu", checkpoint="8bit")
+    else:
+        y = linear_act(*ls, activation="silu", checkpoint="8bit")
+    got = torch.autograd.grad(y, ls, dy)
+    odd = torch.zeros(m, n, dtype=torch.bool)
+    odd[1::2, 5] = odd[1::2, 6] = True
+    assert torch.equal(~y.detach().cpu().isfinite(), odd)
+
+    X8 = _held(X)
+    if gated:
+        A, U = _held(P[:, :n]), _held(P[:, n:])
+        G = torch.cat([D * U * _slope(A, "silu"), D * _act(A, "silu")], 1)
+    else:
+        G = D * _slope(_held(P), "silu")
+    eg = _round(G, BF16) * 1.01 + 16 * _H * G.abs() + 16 * _H * D.abs().repeat(
+        1, outs // n)
+    GM = G.abs() + eg
+    for what, g, want, bound in (
+            ("dx", got[0], G @ W, eg @ W.abs()
+             + (outs + 8) * _H * (GM @ W.abs())),
+            ("dw", got[1], G.t() @ X8, eg.t() @ X8.abs()
+             + (m + 8) * _H * (GM.t() @ X8.abs()))):
+        g = g.cpu().double()
+        lost = want.isnan()
+        assert lost.any() and not lost.all()
+        assert torch.equal(g.isnan(), lost), what
+        bound = bound + _round(want, BF16)
+        worst = ((g - want).abs() / bound)[~lost].max()
+        assert worst <= 1, f"{what}: {worst:.3g} times its bound"
+
+
+@pytest.mark.parametrize("device", _devices())
+@pytest.mark.parametrize("gated", [False, True])
+def test_not_a_number_in_a_row_in_8_bits(gated, device):
+    """A row of NaN stays one: the other rows' results and gradients keep
+    their bits, and the weight's gradient, a sum over all, is NaN."""
+    gen = torch.Generator().manual_seed(3)
+    m, k, n = 80, 72, 50
+    x = torch.randn(m, k, generator=gen).to(BF16).to(device)
+    w = torch.randn(n * (1 + gated), k, generator=gen).to(BF16).to(device)
+    runs = []
+    for spoil in (False, True):
+        v = x.clone()
+        if spoil:
+            v[3, 70] = float("nan")
+        ls = [v.requires_grad_(), w.clone().requires_grad_()]
+        if gated:
+            y = gated_linear(*ls, checkpoint="8bit")
+        else:
+            y = linear_act(*ls, activation="gelu", checkpoint="8bit")
+        runs.append([y.detach(), *torch.autograd.grad(y, ls,
+                                                      torch.ones_like(y))])
+    rows = [i for i in range(m) if i != 3]
+    for a, b in zip(runs[0][:2], runs[1][:2]):
+        assert torch.equal(a[rows], b[rows])
+        assert b[3].isnan().all() and not a.isnan().any()
+    assert runs[1][2].isnan().all() and not runs[0][2].isnan().any()
