@@ -10,7 +10,7 @@ checkpoint format — re-designed for AMD MI355X (gfx950):
 - Sync SGD: bucketed RCCL reduce-scatter + all-gather over xGMI
   (the reduce-scattered segment on each rank *is* the co-located PS
   shard), launched from backward hooks and overlapped with compute.
-- Async SGD: PS shards in host DRAM, pinned hipMemcpyAsync push/pull.
+- Async SGD: PS shards in host DRAM, one copy per shard to push and to pull.
 - Hot ops: hand-written HIP/CDNA4 kernels (MFMA + LDS tiling) in
   ``csrc/kernels``; TCP control plane for bootstrap/coordination.
 

@@ -12,10 +12,14 @@ MI355X-native recast (single node, 8 GPU workers + host-DRAM PS):
   POSIX shared-memory segment (/dev/shm), with per-worker gradient
   slots and seq/ack words.
 - Workers mmap the segment: gradient push is one device→host copy per
-  shard (hipMemcpyAsync through a pinned copy of its size; plain
-  copy on CPU), then a seq bump; parameter pull is one host→device
-  copy. No per-tensor RPC, no serialization — the copy engine moves
-  the bytes over PCIe/IF while compute streams stay busy.
+  shard, then a seq bump; parameter pull is one host→device copy. No
+  per-tensor RPC, no serialization. The copies go to the mapping as it
+  is: a platform may refuse to register memory that exists already, and
+  the next call to the GPU then reports that error as its own. Pinned
+  copies beside it, with the host's copies done by torch's threads, are
+  faster by themselves (ResNet-50, two shards: a pull takes 1.0 ms so
+  and 1.9) but take the cores from the shards' apply threads: 70 ms a
+  step instead of 47 on 16 cores.
 - The PS apply thread spins on seq!=ack, applies the (fused CPU)
   optimizer per worker push, bumps version + global_step (one bump
   per APPLY, the reference's AssignAdd semantics). Staleness
@@ -549,7 +553,7 @@ class AsyncWorkerEngine:
         self._tcp_meta: Dict[int, tuple] = {}
         self._tcp_pver: Dict[int, int] = {}
         # side stream: push/pull copies run off the compute stream (C7's
-        # third stream) so pinned DMA overlaps across shards
+        # third stream)
         self._side = (torch.cuda.Stream(device=device)
                       if device.type == "cuda" else None)
         self.local_step = 0
@@ -651,21 +655,9 @@ class AsyncWorkerEngine:
                 self._tcp_pver[s] = 0
                 if self.device.type == "cuda":
                     pass  # params land via flat_params copy below
-            else:
-                if self.device.type == "cuda":
-                    self._pin_segment(seg, layout)
             self.segs[s] = seg
         self._attached = True
         self.pull()
-
-    def _pin_segment(self, seg: _ShmSeg, layout: _ShmLayout) -> None:
-        """A pinned copy of the shard's size, through which push and pull
-        run as true DMA on the copy engine (hipMemcpyAsync on a
-        side stream).  Allocated, not the mapping registered: a platform
-        may refuse to register memory that exists already, and the next
-        call to the GPU then reports that error as its own."""
-        seg.staging = torch.empty(layout.numel, dtype=seg.dtype,
-                                  pin_memory=True)
 
     # -- engine interface (used by Trainer) ------------------------------
     def broadcast_parameters(self, src: int = 0) -> None:
@@ -711,19 +703,18 @@ class AsyncWorkerEngine:
             if len(self._tcp) == self.num_shards:
                 return
             # mixed shm/tcp: fall through for the shm shards only
-        # push grads to every shard, bump seq (D2H into the pinned copy on
-        # the side stream, then into the shard slot)
+        # push grads to every shard, bump seq (D2H straight into the
+        # shard slot, on the side stream)
         if self._side is not None:
             self._side.wait_stream(torch.cuda.current_stream())
             with torch.cuda.stream(self._side):
                 for s, seg in enumerate(self.segs):
                     if seg is None:
                         continue
-                    seg.staging.copy_(self.flat_grads[s], non_blocking=True)
+                    seg.grads[w].copy_(self.flat_grads[s])
             self._side.synchronize()  # grads visible before the seq bump
             for s, seg in enumerate(self.segs):
                 if seg is not None:
-                    seg.grads[w].copy_(seg.staging)
                     seg.header[_ShmLayout.seq_idx(w)] = self.local_step
         else:
             for s, seg in enumerate(self.segs):
@@ -760,13 +751,11 @@ class AsyncWorkerEngine:
         for s in self._tcp:
             self._tcp_round_trip(s, push=False)
         if self._side is not None:
-            self._side.synchronize()  # the last copies out of the staging
             with torch.cuda.stream(self._side):
                 for s, seg in enumerate(self.segs):
                     if seg is None:
                         continue
-                    seg.staging.copy_(seg.params)
-                    self.flat_params[s].copy_(seg.staging, non_blocking=True)
+                    self.flat_params[s].copy_(seg.params)
             torch.cuda.current_stream().wait_stream(self._side)
         else:
             for s, seg in enumerate(self.segs):
