@@ -127,8 +127,7 @@ void launch_slope_t(Slope s, hipStream_t st) {
   s.strips = s.out == nullptr && s.sums == nullptr ? 0 : (s.n + 255) / 256;
   int more = 0;
   if (s.input.codes != nullptr) {
-    // a block for some 4096 values, 1024 blocks at least where there are so
-    // many
+    // a block for some 4096 values
     const long blocks = (s.input.m * s.input.ldx + 4095) / 4096;
     more = (int)((blocks + s.chunks - 1) / s.chunks);
   }

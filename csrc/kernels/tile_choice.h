@@ -12,9 +12,11 @@
 // and with pre-activations kept, 3 more where one block has the CU and 5 more
 // where they share it; in 8 bits 9 and 8 more.  They are within a tenth or so
 // of what single products take, and chosen so that the rules below choose
-// well: over 91 shapes of the forward pass and 90 of the backward pass, of 70
-// to 16384 rows and widths of 200 to 30528, each with every tile and split
-// measured, the choice is 1.7% and 1.3% slower than the best on average.
+// well: over 82 shapes of the forward pass, each with pre-activations kept and
+// not, and 83 of the backward pass, of 70 to 16384 rows and widths of 200 to
+// 30528, each with every tile and up to eight splits measured, the choice is
+// 1.9% and 1.3% slower than the best on average and 43% and 16% at most
+// (profiles/feed_forward_tile_sweep.txt).
 // A larger tile does more with what it reads; a smaller one leaves fewer CUs
 // without work at the end, and two blocks on a CU write one's results while
 // they multiply the other's.  The choice is the least time of the fullest CU.
@@ -103,8 +105,8 @@ inline TileChoice choose_tile(long m, long n, long k, bool halves, int keep) {
 //   4096 -> 16384           26.6  37.2     33.7  37.8    40.8  38.8
 //   1024 -> 32768           16.5  15.4     20.9  15.6    26.6  16.0
 //   gated, 16384 -> 1024    31.3  23.8     38.7  24.6    45.1  25.4
-// Over 24 shapes of both layers and 1 to 48 rows the choice is 1% slower than
-// the better one.
+// Over 20 shapes of both layers and 1 to 48 rows the choice is 1.7% slower
+// than the better one on average, and 58% at most (1 row of 16384 -> 1024).
 inline double rows_cost(long m, long n, long k, bool gated) {
   const int h = gated ? 2 : 1;
   const long runs = (m + 15) / 16;

@@ -27,10 +27,11 @@
 // half (two of B in LDS) are 2% to 4% slower, steps of 32 in a ring of five
 // 10% to 20%: 64-byte rows cost the L2 as much as 128-byte ones.
 // 4096 x 4096 x 8192 takes 174 us with both operands by k (1582 TFLOP/s), 186
-// with B and 189 with both by rows (185 us on another card, where the library
-// takes 176); without the loads it was 168, and a loop of nothing but matrix
-// instructions on random data runs at 2050 TFLOP/s: the card's power is the
-// bound, the clock falls as the pipe fills.
+// with B and 189 with both by rows; on another card, in a row of 40, 188 (1461
+// TFLOP/s), 190 and 195, where the library takes 210.  Without the loads the
+// 174 were 168, and a loop of nothing but matrix instructions on random data
+// runs at 2050 TFLOP/s: the card's power is the bound, the clock falls as the
+// pipe fills.
 //
 // Loads go from memory to LDS (16 bytes a lane) without passing registers,
 // through buffer descriptors of the tile's own extent: what lies past the last

@@ -7,7 +7,8 @@ is held as e4m3 (1 sign, 4 exponent, 3 mantissa bits) of ``value / 2**e``:
 8.25 bits a value.  ``e`` is the smallest with ``max |value| / 2**e <= 448``,
 e4m3's largest, so scaling is exact and the only rounding is e4m3's, to
 nearest even: at most 2**-4 of a value, or 2**-10 times ``2**e`` where that
-is more.  ``e`` is kept between -118 and 120.
+is more.  ``e`` is kept between -118 and 120.  (On the GPU float32 below
+2**-126 counts as 0, so that such values come back as 0.)
 
 The largest value of a group is taken over its finite ones; infinities and NaN
 come back as NaN, so that a gradient that uses them shows them.  Values that

@@ -12,7 +12,8 @@ refused.
 The backward pass keeps ``x`` and, where there is an activation, the
 pre-activations ``p = x W^T + b`` in the type of ``x``, and computes
 
-    g  = dy * act'(p)              rounded to that type for the products
+    g  = dy * act'(p)              rounded to that type for the products,
+                                   in float16 to infinity past 65504
     dx = g W      dW = g^T x      db = sum over rows of g      dr = dy
 
 db from the unrounded g.  (The gated layer keeps its two projections in 24

@@ -88,7 +88,7 @@ if _hip_sources:
                     "nvcc": ["-O3", "-std=c++17", "--offload-arch=gfx950",
                              "-fgpu-flush-denormals-to-zero",
                              # packed fp32 instructions have given wrong
-                             # results on gfx950; plain ones are as fast here
+                             # results on gfx950, whatever they would save
                              "-Xclang", "-target-feature",
                              "-Xclang", "-packed-fp32-ops"],
                 },

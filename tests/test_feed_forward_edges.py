@@ -5,6 +5,7 @@ lengths at their limits, and every kernel that a choice can lead to."""
 import pytest
 import torch
 
+from rocps.ops.act8 import pack_activation, unpack_activation
 from rocps.ops.gated import gated_linear
 from rocps.ops.linear import linear_act
 from test_feed_forward import _H, _act, _kept8, _round, _slope
@@ -282,3 +283,24 @@ def test_not_a_number_in_a_row_in_8_bits(gated, device):
         assert torch.equal(a[rows], b[rows])
         assert b[3].isnan().all() and not a.isnan().any()
     assert runs[1][2].isnan().all() and not runs[0][2].isnan().any()
+
+
+@pytest.mark.parametrize("device", _devices())
+@pytest.mark.parametrize("t", [BF16, torch.float32])
+def test_pack_the_smallest_values(t, device):
+    """Down to the type's subnormals, where the scale is at its least, 2**-118:
+    off by 2**-4 of the value or 2**-10 of the scale, and on the GPU, where
+    float32 below 2**-126 counts as 0, by that (before and after)."""
+    e = torch.arange(-150, -100).double()
+    v = (2.0 ** e)[:, None] * torch.tensor([1.0, -1.25, 1.5, 1.9375]).double()
+    x = v.reshape(-1, 8).float().to(t)
+    v = x.double()
+    y = unpack_activation(pack_activation(x.to(device))).cpu().double()
+    bound = torch.maximum(v.abs() * 2.0 ** -4, torch.tensor(2.0 ** -128))
+    if device == "cuda":
+        bound = bound + 2 * 2.0 ** -126
+    # a group is a row here, and its scale is its own: at most 448 * 2**e
+    top = v.abs().amax(1, keepdim=True)
+    bound = torch.maximum(bound, top / 224 * 2.0 ** -10)
+    assert ((y - v).abs() <= bound).all()
+    assert torch.equal(y[v == 0], v[v == 0])
